@@ -1,0 +1,486 @@
+"""Measured cases of the paged key-value cache operators: writing new tokens into pages (with MX quantization on the
+way), reading pages back, attention of one new token over the pages, and eviction by accumulated attention weight.
+
+Notation: ``batch`` sequences, ``kv_heads`` heads of ``head_dim`` in the cache, ``group`` query heads for each of them;
+sequence b holds a length between ``lo`` and ``hi``.  The cache holds 16-bit values or MX codes with one scale byte for
+32 elements along the head dimension: keys ``[pages, kv_heads, page, head_dim]`` (4-bit codes two to a byte, the even
+element low) with scales ``[pages, kv_heads, page, head_dim / 32]``, values alike with scales
+``[pages, kv_heads, head_dim / 32, page]``.
+"""
+import math
+
+import torch
+
+own = False
+
+_DT = {"bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def _case(name, op, **kw):
+    base = dict(name=name, op=op, batch=1, kv_heads=8, group=4, head_dim=128, page=64, lo=1, hi=1, fmt="none", dtype="bf16")
+    base.update(kw)
+    return base
+
+
+def listed():
+    return [
+        # a chat's first tokens: one sequence, a few pages; latency is all there is
+        _case("decode short", "decode", page=16, lo=37, hi=37, weights=False, mask=False),
+        # a serving batch in the middle of its answers, lengths all over the range
+        _case("decode batch", "decode", batch=64, lo=65, hi=4096, weights=False, mask=False),
+        # one user with a long document: few rows, a long axis
+        _case("decode long", "decode", lo=131071, hi=131071, page=128, weights=False, mask=False),
+        # the same serving batch at four times the context in 8-bit codes
+        _case("decode mxint8", "decode", batch=32, lo=2048, hi=16384, fmt="mxint8", weights=False, mask=False),
+        # 4-bit codes, eight query heads to a cached one
+        _case("decode mxfp4", "decode", batch=16, group=8, lo=4095, hi=32768, page=32, fmt="mxfp4", weights=False, mask=False),
+        # a head for each query head, left-padded prompts, and the attention weights kept for a later eviction
+        _case("decode weights", "decode", batch=8, kv_heads=16, group=1, head_dim=64, page=16, lo=501, hi=8191, dtype="f16",
+              weights=True, mask=True),
+        # each step of a serving batch writes one token a sequence
+        _case("append step", "append", batch=64, lo=100, hi=2047, new_lo=1, new_hi=1),
+        # prompts of a batch enter an empty cache
+        _case("append prompt", "append", batch=4, lo=0, hi=0, new_lo=1000, new_hi=8191),
+        # the same into 8-bit codes, read back for the prompt's own attention
+        _case("update mxint8", "update", batch=4, lo=0, hi=0, new_lo=517, new_hi=4096, fmt="mxint8"),
+        # a further prompt over what the cache holds: the held part is read back dense
+        _case("gather mxfp8", "gather", batch=8, lo=129, hi=4096, page=32, fmt="mxfp8_e4m3"),
+        # a small budget, one sequence
+        _case("evict small", "evict", page=16, lo=2047, hi=2047, keep=1024, recent=64, first=4),
+        # a batch at a large budget in 8-bit codes; what is left is read back
+        _case("evict large", "evict", batch=8, lo=20001, hi=32768, keep=16384, recent=256, first=4, fmt="mxint8"),
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(["decode", "decode", "append", "update", "gather", "evict"])
+    fmt = rng.choice(["none", "mxint8"] if op == "update" else ["none", "none", "mxint8", "mxfp8_e4m3", "mxfp8_e5m2", "mxfp4"])
+    if op == "append":
+        fmt = "none"
+    kw = dict(batch=_log(rng, 1, 64), kv_heads=rng.choice([1, 2, 4, 8]), group=rng.choice([1, 2, 3, 4, 7, 8, 16]),
+              head_dim=rng.choice([64, 128, 128, 256]), page=rng.choice([8, 16, 32, 64, 128]), fmt=fmt,
+              dtype=rng.choice(["bf16", "bf16", "f16"]))
+    most = min(65536, (1 << 28) // (kw["batch"] * kw["kv_heads"] * kw["head_dim"]))  # slots a sequence may hold at this batch
+    if op == "evict":
+        hi = _log(rng, 64, min(most, 32768))
+        lo = rng.randint(max(1, hi // 2), hi)
+        keep = rng.randint(max(1, hi // 4), hi)
+        kw.update(lo=lo, hi=hi, keep=keep, recent=rng.randint(0, keep // 2), first=rng.randint(0, min(8, keep // 4)))
+    elif op in ("append", "update"):
+        new = _log(rng, 1, min(most // 2, 8192))
+        held = rng.choice([0, _log(rng, 1, min(most // 2, 2048))])
+        kw.update(lo=rng.randint(0, held), hi=held, new_lo=rng.randint(1, new), new_hi=new)
+    else:
+        hi = _log(rng, 1, most if op == "decode" else min(most, 16384))
+        kw.update(lo=rng.randint(1, hi), hi=hi)
+        if op == "decode":
+            kw.update(weights=rng.random() < 0.3, mask=rng.random() < 0.3)
+    c = _case("", op, **kw)
+    del c["name"]
+    return c
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# inputs
+# ---------------------------------------------------------------------------------------------------------------------
+def _spread(lo, hi, n):
+    """n whole numbers from lo to hi, in no order"""
+    return [hi if n == 1 else lo + (hi - lo) * ((i * 7919 + n // 2) % n) // (n - 1) for i in range(n)]
+
+
+def _bytes_per_row(case):
+    """one cached row (one token, one head, keys or values)"""
+    d = case["head_dim"]
+    return {"none": 2 * d, "mxint8": d + d // 32, "mxfp8_e4m3": d + d // 32, "mxfp8_e5m2": d + d // 32, "mxfp4": d // 2 + d // 32}[case["fmt"]]
+
+
+def _float_rows(shape, gen, dev, dtype):
+    """states as projections make them: unit scale, a few channels much larger"""
+    x = torch.randn(shape, generator=gen, device=dev, dtype=torch.float32)
+    big = torch.ones(shape[-1], device=dev)
+    big[:: max(1, shape[-1] // 4)] = 6.0
+    return x.mul_(big).to(dtype)
+
+
+def _code_rows(fmt, shape, gen, dev):
+    """codes of blocks whose largest element is in the top binade, and their scale bytes"""
+    if fmt == "mxint8":
+        c = torch.randn(shape, generator=gen, device=dev).mul_(40.0).round_().clamp_(-128, 127).to(torch.int8)
+        mid = 128  # value = code * 2^(scale - 134)
+    elif fmt == "mxfp4":
+        c = torch.randint(0, 256, (*shape[:-1], shape[-1] // 2), generator=gen, device=dev, dtype=torch.uint8)
+        mid = 125
+    else:
+        c = torch.randint(0, 128, shape, generator=gen, device=dev, dtype=torch.uint8)
+        # exponents near the top of the format as quantized normals have them; the codes that the format reserves left out
+        c = torch.where(c < 64, c // 2 + (64 if fmt == "mxfp8_e5m2" else 80), c).clamp_(max=123 if fmt == "mxfp8_e5m2" else 126)
+        c |= torch.randint(0, 2, shape, generator=gen, device=dev, dtype=torch.uint8) << 7
+        mid = 112 if fmt == "mxfp8_e5m2" else 119
+    s = torch.randint(mid - 1, mid + 2, (*shape[:-1], shape[-1] // 32), generator=gen, device=dev, dtype=torch.uint8)
+    return c, s
+
+
+def prepare(case, seed):
+    dev = torch.device("cuda")
+    gen = torch.Generator(device=dev)
+    gen.manual_seed(seed)
+    dt, op = _DT[case["dtype"]], case["op"]
+    B, Hk, D, P, fmt = case["batch"], case["kv_heads"], case["head_dim"], case["page"], case["fmt"]
+    lens = _spread(case["lo"], case["hi"], B)
+    new = _spread(case.get("new_lo", 0), case.get("new_hi", 0), B)
+    max_len = max(a + b for a, b in zip(lens, new))
+    n_tab = -(-max_len // P)
+    n_pages = B * n_tab + 3
+    s = {"case": case, "max_length": max_len}
+    s["table"] = torch.randperm(n_pages, generator=gen, device=dev)[: B * n_tab].view(B, n_tab).to(torch.int32)
+    s["lengths"] = torch.tensor(lens, dtype=torch.int32, device=dev)
+    shape = (n_pages, Hk, P, D)
+    s["k_scales"] = s["v_scales"] = None
+    if fmt == "none":
+        s["k"], s["v"] = (_float_rows(shape, gen, dev, dt) for _ in range(2))
+    else:
+        s["k"], s["k_scales"] = _code_rows(fmt, shape, gen, dev)
+        s["v"], vs = _code_rows(fmt, shape, gen, dev)
+        s["v_scales"] = vs.transpose(2, 3).contiguous()
+    if op == "decode":
+        s["q"] = torch.randn((B, Hk * case["group"], D), generator=gen, device=dev).to(dt)
+        if case["mask"]:  # left padding: the first slots of a sequence count for nothing
+            pad = torch.tensor([n // 5 for n in lens], device=dev)
+            s["mask"] = torch.zeros((B, 1, max_len), dtype=dt, device=dev).masked_fill_(
+                torch.arange(max_len, device=dev) < pad[:, None, None], torch.finfo(dt).min)
+        if case["weights"]:
+            s["weights"] = torch.rand((B, Hk, n_tab * P), generator=gen, device=dev)
+    elif op in ("append", "update"):
+        n = max(new)
+        # the projections' outputs [batch, tokens, heads * head_dim], seen as heads
+        s["key"], s["value"] = (_float_rows((B, n, Hk, D), gen, dev, dt).transpose(1, 2) for _ in range(2))
+        s["counts"] = torch.tensor(new, dtype=torch.int32, device=dev)
+        s["total"] = s["lengths"] + s["counts"]
+        s["positions"] = torch.full((B, Hk, n_tab * P), -1, dtype=torch.int32, device=dev)
+    elif op == "evict":
+        s["weights"] = torch.rand((B, Hk, n_tab * P), generator=gen, device=dev).pow_(4).mul_(8)
+        # weights that meet: some tokens were never attended to
+        s["weights"].masked_fill_(torch.rand((B, Hk, n_tab * P), generator=gen, device=dev) < 0.3, 0.0)
+        # an earlier eviction has left gaps behind: the positions still rise
+        gaps = torch.randint(1, 3, (B, Hk, n_tab * P), generator=gen, device=dev)
+        s["positions"] = (gaps.cumsum(-1) - 1).to(torch.int32)
+    return s
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# plain form
+# ---------------------------------------------------------------------------------------------------------------------
+def _decode_codes(codes, scales, fmt):
+    """[..., head_dim] values in 32 bits of codes and scale bytes [..., head_dim / 32]"""
+    if fmt == "none":
+        return codes.float()
+    if fmt == "mxint8":
+        x, bias = codes.float(), 134
+    else:
+        if fmt == "mxfp4":
+            codes = torch.stack((codes & 15, codes >> 4), -1).flatten(-2)
+        e, f = {"mxfp4": (2, 1), "mxfp8_e4m3": (4, 3), "mxfp8_e5m2": (5, 2)}[fmt]
+        c = codes.int()
+        man, exp = c & ((1 << f) - 1), (c >> f) & ((1 << e) - 1)
+        mag = torch.ldexp((man + ((exp > 0).int() << f)).float(), exp.clamp(min=1) - ((1 << (e - 1)) - 1) - f)
+        x, bias = torch.where((c >> (e + f)) > 0, -mag, mag), 127
+    return torch.ldexp(x.unflatten(-1, (-1, 32)), (scales.int() - bias)[..., None]).flatten(-2)
+
+
+def _rows(pages, scales, s, fmt, slots_last):
+    """[batch, kv_heads, table slots, head_dim] in 32 bits"""
+    t = s["table"].long()
+    got = pages[t]  # [B, n, Hk, P, D]
+    sc = None
+    if scales is not None:
+        sc = scales[t]
+        sc = sc.transpose(-1, -2) if slots_last else sc
+    return _decode_codes(got, sc, fmt).transpose(1, 2).flatten(2, 3)
+
+
+def _plain_gather(s, lengths, n, dt):
+    fmt = s["case"]["fmt"]
+    k = _rows(s["k"], s["k_scales"], s, fmt, False)[:, :, :n]
+    v = _rows(s["v"], s["v_scales"], s, fmt, True)[:, :, :n]
+    held = (torch.arange(n, device=k.device) < lengths[:, None])[:, None, :, None]
+    return torch.where(held, k, 0.0).to(dt), torch.where(held, v, 0.0).to(dt)
+
+
+def _plain_decode(s):
+    c = s["case"]
+    n, hk, dt = s["max_length"], c["kv_heads"], _DT[c["dtype"]]
+    k = _rows(s["k"], s["k_scales"], s, c["fmt"], False)[:, :, :n]
+    q = s["q"].float().unflatten(1, (hk, -1))  # [B, Hk, G, D]
+    x = torch.matmul(q, k.transpose(-1, -2)) * c["head_dim"] ** -0.5
+    del k
+    if "mask" in s:
+        x = x + s["mask"].float()[:, :, None]
+    held = (torch.arange(n, device=x.device) < s["lengths"][:, None])[:, None, None]
+    x = torch.where(held, x, -math.inf)
+    top = x.amax(-1, keepdim=True)
+    p = torch.exp(x - torch.where(top == -math.inf, 0.0, top))
+    p = p / p.sum(-1, keepdim=True).clamp(min=1e-30)
+    v = _rows(s["v"], s["v_scales"], s, c["fmt"], True)[:, :, :n]
+    v = torch.where(held[:, :, 0, :, None], v, 0.0)
+    out = torch.matmul(p, v).flatten(1, 2).to(dt)
+    if "weights" in s:
+        s["weights"][:, :, :n] += p.sum(2)
+        return out, s["weights"]
+    return out
+
+
+def _mxint8_codes(x):
+    """codes and scale bytes of blocks of 32: the exponent is the ceiling of log2 of the largest element, a logarithm of
+    the tensor's own type"""
+    b = x.unflatten(-1, (-1, 32))
+    top = b.abs().amax(-1).clamp(min=torch.finfo(x.dtype).tiny)
+    k = torch.ceil(torch.log2(top.float()).to(x.dtype)).int()
+    codes = torch.round(torch.ldexp(b.float(), 7 - k[..., None])).clamp(-128, 127)
+    return codes.flatten(-2).to(torch.int8), (k + 127).clamp(0, 255).to(torch.uint8)
+
+
+def _plain_append(s):
+    c, n = s["case"], s["key"].shape[2]
+    j = torch.arange(n, device=s["key"].device)
+    b, t = torch.nonzero(j < s["counts"][:, None], as_tuple=True)
+    slot = s["lengths"][b].long() + t
+    page, at = s["table"][b, slot // c["page"]].long(), slot % c["page"]
+    key, value = s["key"][b, :, t], s["value"][b, :, t]  # [tokens, Hk, D]
+    if c["fmt"] == "none":
+        s["k"][page, :, at], s["v"][page, :, at] = key, value
+    else:
+        s["k"][page, :, at], s["k_scales"][page, :, at] = _mxint8_codes(key)
+        s["v"][page, :, at], s["v_scales"][page, :, :, at] = _mxint8_codes(value)
+    s["positions"][b, :, slot] = slot[:, None].int()
+
+
+def _plain_evict(s):
+    c, w, pos = s["case"], s["weights"], s["positions"]
+    keep, n = c["keep"], w.shape[-1]
+    slot = torch.arange(n, device=w.device)
+    held = (slot < s["lengths"][:, None])[:, None]
+    newest = torch.where(held, pos, -1).amax(-1, keepdim=True)
+    safe = (pos < c["first"]) | (pos > newest - c["recent"])
+    rank = torch.where(held, torch.where(safe, math.inf, w), -math.inf)
+    order = torch.sort(rank, dim=-1, descending=True, stable=True).indices  # ties: the lowest slot first
+    kept = torch.zeros_like(w, dtype=torch.bool).scatter_(2, order[..., :keep], True) & held
+    # the j-th free slot below `keep` takes the j-th kept token behind it
+    free, more = ~kept & (slot < keep), kept & (slot >= keep)
+    behind = torch.zeros_like(order).scatter_(2, torch.where(more, more.long().cumsum(-1) - 1, n - 1), slot.expand_as(order).contiguous())
+    src = torch.where(free, torch.gather(behind, 2, (free.long().cumsum(-1) - 1).clamp(min=0)), slot)
+    length = s["lengths"].clamp(max=keep)
+    live = (slot < length[:, None])[:, None].expand_as(w)
+    src = torch.where(live, src, slot)
+    new_w, new_pos = torch.where(live, w.gather(2, src), 0.0), torch.where(live, pos.gather(2, src), -1)
+    b, h, t = torch.nonzero(live & (src != slot), as_tuple=True)
+    f = src[b, h, t]
+    table, page = s["table"].long(), c["page"]
+    fp, fa, tp, ta = table[b, f // page], f % page, table[b, t // page], t % page
+    s["k"][tp, h, ta], s["v"][tp, h, ta] = s["k"][fp, h, fa], s["v"][fp, h, fa]
+    if c["fmt"] != "none":
+        s["k_scales"][tp, h, ta] = s["k_scales"][fp, h, fa]
+        s["v_scales"][tp, h, :, ta] = s["v_scales"][fp, h, :, fa]
+    return new_w, new_pos, length
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# one pass
+# ---------------------------------------------------------------------------------------------------------------------
+def _run_own(s):
+    from mase_amd.quantized import functional as F
+
+    c, dt = s["case"], _DT[s["case"]["dtype"]]
+    pool = dict(kv_format=None if c["fmt"] == "none" else c["fmt"], k_scales=s["k_scales"], v_scales=s["v_scales"])
+    if c["op"] == "decode":
+        out = F.paged_attention_decode(s["q"], s["k"], s["v"], s["table"], s["lengths"], s["max_length"],
+                                       mask=s.get("mask"), weights=s.get("weights"), **pool)
+        return (out, s["weights"]) if "weights" in s else out
+    if c["op"] in ("append", "update"):
+        F.paged_kv_append(s["key"], s["value"], s["k"], s["v"], s["table"], s["lengths"], counts=s["counts"],
+                          positions=s["positions"], **pool)
+        if c["op"] == "append":
+            return s["k"], s["v"], s["positions"]
+        return (*F.paged_kv_gather(s["k"], s["v"], s["table"], s["total"], s["max_length"], dtype=dt, **pool), s["positions"])
+    if c["op"] == "gather":
+        return F.paged_kv_gather(s["k"], s["v"], s["table"], s["lengths"], s["max_length"], dtype=dt, **pool)
+    w, pos, length = F.paged_kv_evict(s["k"], s["v"], s["table"], s["lengths"], s["weights"], s["positions"], s["max_length"],
+                                      c["keep"], recent=c["recent"], first=c["first"], **pool)
+    n = min(c["keep"], s["max_length"])
+    rows = (s["k"], s["v"]) if c["fmt"] == "none" else F.paged_kv_gather(s["k"], s["v"], s["table"], length, n, dtype=dt, **pool)
+    return w, pos, length, *rows
+
+
+def run(state):
+    s = state
+    if own:
+        return _run_own(s)
+    c, dt = s["case"], _DT[s["case"]["dtype"]]
+    if c["op"] == "decode":
+        return _plain_decode(s)
+    if c["op"] in ("append", "update"):
+        _plain_append(s)
+        if c["op"] == "append":
+            return s["k"], s["v"], s["positions"]
+        return (*_plain_gather(s, s["total"], s["max_length"], dt), s["positions"])
+    if c["op"] == "gather":
+        return _plain_gather(s, s["lengths"], s["max_length"], dt)
+    w, pos, length = _plain_evict(s)
+    n = min(c["keep"], s["max_length"])
+    rows = (s["k"], s["v"]) if c["fmt"] == "none" else _plain_gather(s, length, n, dt)
+    return w, pos, length, *rows
+
+
+def work(case):
+    """bytes read once and written once, and the products' operations"""
+    B, Hk, D, G = case["batch"], case["kv_heads"], case["head_dim"], case["group"]
+    lens, new = _spread(case["lo"], case["hi"], B), _spread(case.get("new_lo", 0), case.get("new_hi", 0), B)
+    row, tokens, op = 2 * _bytes_per_row(case), sum(lens), case["op"]
+    dense = 4 * D  # keys and values of one token and head in 16 bits
+    top = max(a + b for a, b in zip(lens, new))
+    flops = 0.0
+    if op == "decode":
+        n = tokens * Hk * row + 2 * B * Hk * G * D * 2 + tokens * Hk * 8 * case["weights"] + tokens * 2 * case["mask"]
+        flops = 4.0 * tokens * Hk * G * D
+    elif op == "gather":
+        n = tokens * Hk * row + B * Hk * top * dense
+    elif op in ("append", "update"):
+        n = sum(new) * Hk * (dense + row + 4)
+        if op == "update":
+            n += tokens * Hk * row + B * Hk * top * dense
+    else:
+        keep = case["keep"]
+        moved = sum(max(0, x - keep) * keep / x for x in lens if x)
+        slots = -(-top // case["page"]) * case["page"]
+        n = tokens * Hk * 8 + B * slots * Hk * 8 + 2 * moved * Hk * row
+        if case["fmt"] != "none":
+            n += sum(min(x, keep) for x in lens) * Hk * row + B * Hk * min(keep, top) * dense
+    return {"bytes": float(n), "flops": flops}
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# the definitions in 64 bits, sequence by sequence
+# ---------------------------------------------------------------------------------------------------------------------
+_E4M3 = [(-1.0 if c & 128 else 1.0) * ((c & 7) * 2.0 ** -9 if not c & 120 else (8 + (c & 7)) * 2.0 ** ((c >> 3 & 15) - 10)) for c in range(256)]
+_E5M2 = [(-1.0 if c & 128 else 1.0) * ((c & 3) * 2.0 ** -16 if not c & 124 else (4 + (c & 3)) * 2.0 ** ((c >> 2 & 31) - 17)) for c in range(256)]
+_E2M1 = [0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, -0.0, -0.5, -1.0, -1.5, -2.0, -3.0, -4.0, -6.0]
+
+
+def _sequence64(s, b, n):
+    """keys and values [kv_heads, n, head_dim] of sequence b"""
+    c, got = s["case"], []
+    pages = s["table"][b].tolist()[: -(-n // c["page"])]
+    for name in ("k", "v"):
+        x = torch.cat([s[name][p] for p in pages], 1)[:, :n] if pages else s[name][0][:, :0]
+        if c["fmt"] == "none":
+            got.append(x.double())
+            continue
+        if c["fmt"] == "mxint8":
+            x = x.double() / 128
+        elif c["fmt"] == "mxfp4":
+            tab = torch.tensor(_E2M1, dtype=torch.float64, device=x.device)
+            wide = x.new_empty((*x.shape[:-1], 2 * x.shape[-1]))
+            wide[..., 0::2], wide[..., 1::2] = x % 16, x // 16
+            x = tab[wide.long()]
+        else:
+            x = torch.tensor(_E4M3 if c["fmt"] == "mxfp8_e4m3" else _E5M2, dtype=torch.float64, device=x.device)[x.long()]
+        if name == "k":
+            sc = torch.cat([s["k_scales"][p] for p in pages], 1)[:, :n]
+        else:
+            sc = torch.cat([s["v_scales"][p] for p in pages], 2)[:, :, :n].transpose(1, 2)
+        got.append(x * torch.exp2(sc.double() - 127).repeat_interleave(32, -1))
+    return got
+
+
+def _dense64(s, lengths, n):
+    c = s["case"]
+    out = torch.zeros((2, c["batch"], c["kv_heads"], n, c["head_dim"]), dtype=torch.float64, device=s["k"].device)
+    for b, m in enumerate(lengths):
+        if m:
+            out[0, b, :, :m], out[1, b, :, :m] = _sequence64(s, b, m)
+    return out[0], out[1]
+
+
+def _quantized64(x):
+    """the MXINT8 values of x's blocks of 32 along the last dimension"""
+    y = x.double().reshape(-1, 32)
+    top = y.abs().max(1, keepdim=True).values.clamp_min(float(torch.finfo(x.dtype).tiny))
+    step = torch.exp2(torch.ceil(torch.log2(top).to(x.dtype).double()) - 7)
+    return ((y / step).round().clamp(-128, 127) * step).reshape(x.shape)
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    op, P, Hk = case["op"], case["page"], case["kv_heads"]
+    lens = s["lengths"].tolist()
+    if op == "gather":
+        return _dense64(s, lens, s["max_length"])
+    if op == "decode":
+        out = torch.zeros(s["q"].shape, dtype=torch.float64, device=s["q"].device)
+        acc = s["weights"].double() if case["weights"] else None
+        for b, m in enumerate(lens):
+            if not m:
+                continue
+            k, v = _sequence64(s, b, m)
+            for h in range(Hk):
+                rows = slice(h * case["group"], (h + 1) * case["group"])
+                x = s["q"][b, rows].double() @ k[h].T / math.sqrt(case["head_dim"])
+                if case["mask"]:
+                    x += s["mask"][b, 0, :m].double()
+                p = torch.softmax(x, -1)
+                out[b, rows] = p @ v[h]
+                if acc is not None:
+                    acc[b, h, :m] += p.sum(0)
+        return out if acc is None else (out, acc)
+    if op in ("append", "update"):
+        if op == "update":
+            k, v = _dense64(s, lens, s["max_length"])
+        else:
+            k, v = s["k"].double(), s["v"].double()
+        for b, (m, n) in enumerate(zip(lens, s["counts"].tolist())):
+            key, value = s["key"][b, :, :n], s["value"][b, :, :n]
+            if op == "update":
+                quant = _quantized64 if case["fmt"] == "mxint8" else torch.Tensor.double
+                k[b, :, m:m + n], v[b, :, m:m + n] = quant(key), quant(value)
+                continue
+            done = 0
+            while done < n:  # page by page
+                p, at = int(s["table"][b, (m + done) // P]), (m + done) % P
+                some = min(P - at, n - done)
+                k[p, :, at:at + some], v[p, :, at:at + some] = key[:, done:done + some], value[:, done:done + some]
+                done += some
+        return k, v, None
+    keep, n = case["keep"], s["weights"].shape[-1]
+    w, pos = s["weights"].double().cpu(), s["positions"].cpu()
+    new_w = torch.zeros_like(w)
+    moves = []
+    for b, m in enumerate(lens):
+        for h in range(Hk):
+            at = pos[b, h, :m]
+            rank = torch.where((at < case["first"]) | (at > int(at.max()) - case["recent"]), math.inf, w[b, h, :m])
+            best = torch.argsort(-rank, stable=True)[:keep].sort().values
+            inside = best[best < keep]
+            src = torch.arange(min(m, keep))
+            free = torch.ones(len(src), dtype=torch.bool)
+            free[inside] = False
+            if m > keep:
+                src[free] = best[best >= keep]
+            new_w[b, h, : len(src)] = w[b, h, src]
+            moves.append((b, h, src.to(s["k"].device)))
+    if case["fmt"] != "none":
+        top = min(keep, s["max_length"])
+        k, v = _dense64(s, lens, s["max_length"])
+        out = [torch.zeros((*k.shape[:2], top, k.shape[3]), dtype=torch.float64, device=k.device) for _ in range(2)]
+        for b, h, src in moves:
+            out[0][b, h, : len(src)], out[1][b, h, : len(src)] = k[b, h, src], v[b, h, src]
+    else:
+        out = [s["k"].double(), s["v"].double()]
+        for b, h, src in moves:
+            page = s["table"][b].long()
+            to = torch.arange(len(src), device=src.device)
+            for o, name in zip(out, ("k", "v")):
+                o[page[to // P], h, to % P] = s[name][page[src // P], h, src % P].double()
+    return new_w, None, None, out[0], out[1]
