@@ -62,7 +62,7 @@ def draw(rng):
     if op == "append":
         fmt = "none"
     kw = dict(batch=_log(rng, 1, 64), kv_heads=rng.choice([1, 2, 4, 8]), group=rng.choice([1, 2, 3, 4, 7, 8, 16]),
-              head_dim=rng.choice([64, 128, 128, 256]), page=rng.choice([8, 16, 32, 64, 128]), fmt=fmt,
+              head_dim=rng.choice([64, 128, 128, 256]), page=rng.choice([16, 32, 64, 128]), fmt=fmt,
               dtype=rng.choice(["bf16", "bf16", "f16"]))
     most = min(65536, (1 << 28) // (kw["batch"] * kw["kv_heads"] * kw["head_dim"]))  # slots a sequence may hold at this batch
     if op == "evict":
