@@ -30,6 +30,10 @@
  *   mase_add_rmsnorm_mxint  models/llama/modeling_llama.py:901-905 (residual addition, then the norm as above)
  *   mase_attn_softmax_mx    nn/quantized/modules/llama/attention.py:363-392 (scores -> quantized probabilities)
  *   mase_attention_causal   models/llama/modeling_llama.py:362-480 (the attention core on unquantized q, k, v)
+ *   mase_paged_kv_append, mase_paged_kv_gather   nn/quantized/functional/kvcache.py:8-43 followed by past_key_value.update
+ *                           (nn/quantized/modules/llama/attention.py:182-187), the codes held in pages
+ *   mase_paged_attention_decode   the attention core on such a cache for one new token (models/llama/modeling_llama.py:362-480)
+ *   mase_paged_kv_evict     no counterpart in the reference
  *   mase_mx_unpack          nn/quantizers/mxint/fake.py:59-80, nn/quantizers/mxfp/fake.py:75-104 (compose_*)
  *   mase_mxfp_pack(_tiled), mase_mxfp_tile_codes, mase_gemm_mxfp_scaled, mase_gemm_mxfp4_scaled_tiled
  *                           nn/quantized/modules/linear.py:877-895 (LinearMXFP.forward on
@@ -403,6 +407,96 @@ int mase_transpose16(const void* in, void* out, size_t batch_outer, size_t batch
 int mase_rope(const void* x, const void* cos, const void* sin, void* out, size_t B, size_t H, size_t T, size_t D,
               size_t x_stride_b, size_t x_stride_h, size_t x_stride_t, size_t cs_stride_b, size_t cs_stride_t, int dtype,
               void* stream);
+
+/*
+ * Paged key-value cache: fixed-size pages of a pool hold the keys and values of many sequences; a sequence's slot t is row
+ * t % page_size of page page_table[sequence][t / page_size].  What the reference's attention modules keep through
+ * past_key_value.update (nn/quantized/modules/llama/attention.py:182-187) and the MX quantizers of its cache
+ * (nn/quantized/functional/kvcache.py:8-43) are held here as codes instead of fake-quantized 16-bit values.
+ *
+ * Formats (MX blocks of 32 along the head dimension, one scale byte each; byte 255: the block reads as NaN):
+ *   MASE_KV_16BIT      states of `dtype` (bf16 or fp16) as they are
+ *   MASE_KV_MXINT8     int8 codes, value code * 2^(scale - 134): the values of mase_mxint_qdq (8 bits, 8-bit scales);
+ *                      its NaN blocks (a non-finite element, an exponent beyond dtype) have scale 255
+ *   MASE_KV_MXFP8_E4M3, MASE_KV_MXFP8_E5M2, MASE_KV_MXFP4 (e2m1, two to a byte, the even element low)
+ *                      codes and scales of mase_mxfp_pack, value element * 2^(scale - 127)
+ * Pages: k, v [num_pages][kv_heads][page_size][head_dim] with byte strides of page, head and slot (rows contiguous;
+ * 16-bit rows and 8-bit rows 16-byte aligned, strides multiples of 16); k_scales [num_pages][kv_heads][page_size]
+ * [head_dim / 32], v_scales [num_pages][kv_heads][head_dim / 32][page_size], both contiguous, 8-byte aligned.
+ * head_dim 64, 128 or 256; page_size a power of two from 16 to 4096.  page_table [batch][table_pages], rows table_stride
+ * entries apart.
+ * Lengths, slots and page numbers are read on the device: a length counts for at most max_length and what the table holds,
+ * and a page number outside the pool is never followed (its slots are absent: nothing is written there, and readers pass
+ * over them).  Pages past a sequence's length may hold anything.  Calls that write to a page must not overlap with others
+ * on it, and within one call no slot may be named twice.
+ */
+#define MASE_KV_16BIT 0
+#define MASE_KV_MXINT8 1
+#define MASE_KV_MXFP8_E4M3 2
+#define MASE_KV_MXFP8_E5M2 3
+#define MASE_KV_MXFP4 4
+typedef struct mase_paged_kv {
+  void* k;
+  void* v;
+  uint8_t* k_scales; /* NULL with MASE_KV_16BIT */
+  uint8_t* v_scales;
+  const int32_t* page_table;
+  size_t num_pages, page_size, kv_heads, head_dim;
+  size_t batch, table_pages, table_stride;
+  size_t k_stride_page, k_stride_head, k_stride_slot; /* bytes */
+  size_t v_stride_page, v_stride_head, v_stride_slot;
+  int32_t format; /* MASE_KV_* */
+  int32_t dtype;  /* MASE_DT_BF16 or MASE_DT_F16: type of the states written, read and attended with */
+} mase_paged_kv;
+
+/* Writes new tokens: token j < counts[b] (counts NULL: all `tokens`) of sequence b goes to slot starts[b] + j.  key, value
+ * [batch][kv_heads][tokens][head_dim] of `dtype` by element strides of batch, head and token (rows contiguous, 16-byte
+ * aligned, strides multiples of 8).  MX formats quantize on the way with the arithmetic of the functions named above;
+ * log2_tab is the table of `dtype` for MXINT8, the fp32 table for the MXFP formats, unused (may be NULL) for 16 bits.
+ * positions (optional) [batch][kv_heads][...] int32 by element strides of batch and head: entry slot becomes
+ * first_positions[b] + j (first_positions NULL: starts[b] + j), for the eviction below. */
+int mase_paged_kv_append(const mase_paged_kv* cache, const void* key, const void* value, size_t tokens, size_t key_stride_b,
+                         size_t key_stride_h, size_t key_stride_t, size_t value_stride_b, size_t value_stride_h,
+                         size_t value_stride_t, const int32_t* starts, const int32_t* counts, int32_t* positions,
+                         size_t pos_stride_b, size_t pos_stride_h, const int32_t* first_positions,
+                         const uint32_t* log2_tab, void* stream);
+
+/* Reads sequences back dense: key, value [batch][kv_heads][max_length][head_dim] of `dtype`, contiguous, 16-byte aligned;
+ * slots from lengths[b] on (and absent ones) become zero. */
+int mase_paged_kv_gather(const mase_paged_kv* cache, const int32_t* lengths, size_t max_length, void* key, void* value,
+                         void* stream);
+
+/* Attention of one new token per sequence over its cached slots: x = scaling * (q . k) + mask, p = softmax(x),
+ * out = sum p v for q, out [batch][heads][head_dim] of `dtype` (q by element strides of batch and head, multiples of 8,
+ * rows 16-byte aligned; out contiguous); query head h reads cached head h / (heads / kv_heads).  Scores, softmax statistics
+ * and sums are fp32; probabilities are rounded to `dtype` for the product with the values.
+ * mask (optional): added to the scores of all heads, [batch][max_length] of mask_dtype (the cache's dtype or fp32) with an
+ * element stride of batch (0: one row for all); a slot whose mask is -inf is left out whatever its keys and values hold.
+ * A row without a slot gives zeros.
+ * weights (optional, fp32) [batch][kv_heads][...] by element strides of batch and head: entry t grows by the probabilities
+ * of slot t summed over the query heads of its cached head, in a fixed order.
+ * The cache is split over its length; the parts (and with weights the scores) pass through `workspace`,
+ * mase_paged_attention_decode_workspace_bytes() bytes, 16-byte aligned (0 bytes: NULL will do). */
+size_t mase_paged_attention_decode_workspace_bytes(size_t batch, size_t heads, size_t kv_heads, size_t head_dim,
+                                                   size_t max_length, int with_weights);
+int mase_paged_attention_decode(const mase_paged_kv* cache, const void* q, size_t q_stride_b, size_t q_stride_h, size_t heads,
+                                const int32_t* lengths, size_t max_length, float scaling, const void* mask, int mask_dtype,
+                                size_t mask_stride_b, float* weights, size_t w_stride_b, size_t w_stride_h, void* out,
+                                void* workspace, size_t workspace_bytes, void* stream);
+
+/* Eviction by accumulated attention weight: every cached head of a sequence longer than `keep` slots keeps `keep` of them:
+ * those at a position below `first` or above (largest position - recent), then those of the largest weight; ties (and
+ * more than `keep` protected ones) go to the lowest slot, NaN counts as the smallest weight.  Kept slots below `keep` stay
+ * where they are; the free ones there, in order, take the kept slots behind them, in order (attention does not depend on
+ * the order of its slots; positions tell where a token stood).  first + recent <= keep.
+ * weights, positions: [batch][kv_heads][capacity] contiguous; weights_out, positions_out likewise (other memory): what
+ * belongs to the slots after the eviction, then 0 and -1; lengths_out[b] = min(lengths[b], keep).  Pages must belong to one
+ * sequence only.  workspace: mase_paged_kv_evict_workspace_bytes() bytes, 16-byte aligned. */
+size_t mase_paged_kv_evict_workspace_bytes(size_t batch, size_t kv_heads, size_t keep);
+int mase_paged_kv_evict(const mase_paged_kv* cache, const int32_t* lengths, size_t max_length, const float* weights,
+                        const int32_t* positions, size_t capacity, size_t keep, size_t recent, size_t first,
+                        float* weights_out, int32_t* positions_out, int32_t* lengths_out, void* workspace,
+                        size_t workspace_bytes, void* stream);
 
 /* test/diagnostic helpers (host only, no device work) */
 uint32_t mase_isclose_zero_threshold_bits(int dtype); /* largest |x| (fp32 bits) that isclose(x, 0) accepts */

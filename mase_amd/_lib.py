@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_double, c_float, c_int, c_size_t, c_uint32, c_void_p
+from ctypes import c_char_p, c_double, c_float, c_int, c_int32, c_size_t, c_uint32, c_void_p
 
 import torch
 
@@ -19,8 +19,20 @@ LOG2_TABLE_WORDS = 576
 BLOCK_FP_STATIC_MAX_TILES = 1 << 20
 
 
+KV_FORMATS = {None: 0, "mxint8": 1, "mxfp8_e4m3": 2, "mxfp8_e5m2": 3, "mxfp4": 4}
+
+
 class MaseAmdError(RuntimeError):
     pass
+
+
+class PagedKv(ctypes.Structure):
+    """``mase_paged_kv`` of the C ABI"""
+    _fields_ = ([(n, c_void_p) for n in ("k", "v", "k_scales", "v_scales", "page_table")]
+                + [(n, c_size_t) for n in ("num_pages", "page_size", "kv_heads", "head_dim", "batch", "table_pages",
+                                           "table_stride", "k_stride_page", "k_stride_head", "k_stride_slot",
+                                           "v_stride_page", "v_stride_head", "v_stride_slot")]
+                + [("format", c_int32), ("dtype", c_int32)])
 
 
 # name -> (restype, argtypes); one entry per symbol declared in include/mase_amd.h
@@ -86,6 +98,15 @@ SIGNATURES = {
     "mase_gemm_mxfp4_scaled_tiled": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
                                              c_size_t, c_size_t, c_int, c_int, c_void_p]),
     "mase_gemm_mxfp_scaled": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_size_t, c_size_t, c_size_t, c_int, c_int, c_void_p]),
+    "mase_paged_kv_append": (c_int, [c_void_p, c_void_p, c_void_p] + [c_size_t] * 7 + [c_void_p, c_void_p, c_void_p, c_size_t, c_size_t,
+                                     c_void_p, c_void_p, c_void_p]),
+    "mase_paged_kv_gather": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p, c_void_p, c_void_p]),
+    "mase_paged_attention_decode_workspace_bytes": (c_size_t, [c_size_t] * 5 + [c_int]),
+    "mase_paged_attention_decode": (c_int, [c_void_p, c_void_p, c_size_t, c_size_t, c_size_t, c_void_p, c_size_t, c_float, c_void_p,
+                                            c_int, c_size_t, c_void_p, c_size_t, c_size_t, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "mase_paged_kv_evict_workspace_bytes": (c_size_t, [c_size_t] * 3),
+    "mase_paged_kv_evict": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p, c_void_p] + [c_size_t] * 4
+                            + [c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "mase_isclose_zero_threshold_bits": (c_uint32, [c_int]),
     "mase_round_scalar_to_dtype": (c_float, [c_double, c_int]),
 }

@@ -100,4 +100,37 @@ __device__ __forceinline__ void mxfp_elements(const float* x, int state, int sh,
   }
 }
 
+// largest magnitude (fp32 bits) of the flushed elements of one 16-byte input vector
+template <int DTI>
+__device__ __forceinline__ uint32_t vec_flushed_absmax(const uint4& v) {
+  const uint32_t m = vec_absmax_bits<DTI>(v);
+  return ((m & 0x7F800000u) == 0) ? 0u : m;  // a subnormal maximum means every element is flushed
+}
+
+// codes that the OCP element formats reserve, and a code halved (see the packing kernels)
+template <int E, int F>
+__device__ __forceinline__ uint32_t halve_code(uint32_t c) {
+  const uint32_t sgn = c & (1u << (E + F));
+  uint32_t e = (c >> F) & ((1u << E) - 1u);
+  uint32_t f = c & ((1u << F) - 1u);
+  if (e >= 2) {
+    e -= 1;
+  } else {
+    uint32_t v = (e == 1) ? ((1u << F) + f) : f;
+    uint32_t q = (v >> 1) + ((v & 1u) & ((v >> 1) & 1u));  // round half to even
+    if (q == (1u << F)) { e = 1; f = 0; }
+    else { e = 0; f = q; }
+  }
+  return sgn | (e << F) | f;
+}
+
+template <int E, int F>
+__device__ __forceinline__ bool code_is_reserved(uint32_t c) {
+  const uint32_t e = (c >> F) & ((1u << E) - 1u);
+  const uint32_t f = c & ((1u << F) - 1u);
+  if constexpr (E == 4 && F == 3) return e == 15u && f == 7u;  // OCP e4m3: NaN
+  if constexpr (E == 5 && F == 2) return e == 31u;             // OCP e5m2: Inf / NaN
+  return false;
+}
+
 }  // namespace mase

@@ -1,0 +1,599 @@
+// Paged key-value cache for gfx950: writing new tokens (with MX quantization on the way), reading sequences back dense, and
+// eviction by accumulated attention weight.  What the reference's attention modules do through
+// kv_cache_mxfp / kv_cache_mxint and past_key_value.update (nn/quantized/functional/kvcache.py:8-43,
+// nn/quantized/modules/llama/attention.py:182-187), with the codes themselves held in pages.  All of it is bound by HBM.
+#include "paged_kv.hpp"
+#include "mxfp_core.hpp"
+#include "mxint_core.hpp"
+
+namespace mase {
+
+int paged_kv_params(const mase_paged_kv* c, PagedKv& p) {
+  if (c == nullptr || c->k == nullptr || c->v == nullptr || c->page_table == nullptr) return MASE_ERR_NULL;
+  if (c->dtype != MASE_DT_BF16 && c->dtype != MASE_DT_F16) return MASE_ERR_DTYPE;
+  if (c->format < MASE_KV_16BIT || c->format > MASE_KV_MXFP4) return MASE_ERR_PARAM;
+  const bool packed = c->format != MASE_KV_16BIT;
+  if (packed && (c->k_scales == nullptr || c->v_scales == nullptr)) return MASE_ERR_NULL;
+  if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return MASE_ERR_SHAPE;
+  const size_t ps = c->page_size;
+  if (ps < 16 || ps > 4096 || (ps & (ps - 1)) != 0) return MASE_ERR_SHAPE;
+  // slots are counted in 32 bits on the device, grids have at most 65535 sequences and heads
+  if (c->num_pages == 0 || c->num_pages > 0x7FFFFFFFu || c->table_pages == 0 || c->table_pages > 0x7FFFFFFFu / ps ||
+      c->table_stride < c->table_pages || c->batch > 65535 || c->kv_heads == 0 || c->kv_heads > 65535)
+    return MASE_ERR_SHAPE;
+  const size_t strides[6] = {c->k_stride_page, c->k_stride_head, c->k_stride_slot,
+                             c->v_stride_page, c->v_stride_head, c->v_stride_slot};
+  for (size_t s : strides)
+    if (s % 16 != 0) return MASE_ERR_ALIGN;
+  const size_t row = kv_row_bytes(c->format, c->head_dim);
+  // a page's rows of one head lie within 32-bit byte offsets
+  if (c->k_stride_slot < row || c->v_stride_slot < row || c->k_stride_slot > 0x7FFFFFFFu / ps ||
+      c->v_stride_slot > 0x7FFFFFFFu / ps)
+    return MASE_ERR_SHAPE;
+  if (!aligned16(c->k) || !aligned16(c->v)) return MASE_ERR_ALIGN;
+  if (packed && (((uintptr_t)c->k_scales | (uintptr_t)c->v_scales) & 7u) != 0) return MASE_ERR_ALIGN;
+  if (((uintptr_t)c->page_table & 3u) != 0) return MASE_ERR_ALIGN;
+  p.k = (unsigned char*)c->k;
+  p.v = (unsigned char*)c->v;
+  p.ks = c->k_scales;
+  p.vs = c->v_scales;
+  p.table = c->page_table;
+  p.table_stride = c->table_stride;
+  p.k_page = c->k_stride_page; p.k_head = c->k_stride_head; p.k_slot = (uint32_t)c->k_stride_slot;
+  p.v_page = c->v_stride_page; p.v_head = c->v_stride_head; p.v_slot = (uint32_t)c->v_stride_slot;
+  p.num_pages = (int)c->num_pages;
+  p.page_shift = __builtin_ctzll((unsigned long long)ps);
+  p.table_pages = (int)c->table_pages;
+  p.heads = (int)c->kv_heads;
+  return MASE_OK;
+}
+
+namespace {
+
+// first scale byte of a row of keys, and of a slot's column of values (the other bytes follow at 1 and at page_size)
+template <int D>
+__device__ __forceinline__ size_t key_scale_at(const PagedKv& p, int page, int head, int row) {
+  return ((((size_t)page * p.heads + head) << p.page_shift) + row) * (D / 32);
+}
+template <int D>
+__device__ __forceinline__ size_t value_scale_at(const PagedKv& p, int page, int head, int row) {
+  return ((((size_t)page * p.heads + head) * (D / 32)) << p.page_shift) + row;
+}
+
+// -------------------------------------------------------------------------------------------------
+// append
+// -------------------------------------------------------------------------------------------------
+struct AppendParams {
+  PagedKv c;
+  const unsigned char* key;
+  const unsigned char* value;
+  size_t k_sb, k_sh, k_st, v_sb, v_sh, v_st;  // byte strides
+  const int32_t* starts;
+  const int32_t* counts;
+  int32_t* positions;
+  size_t pos_sb, pos_sh;
+  const int32_t* first_positions;
+  int tokens;
+  uint32_t items;  // tokens * heads * D / 8
+  MxintParams mxint;
+  MxfpParams mxfp;
+};
+
+// 8 elements to their codes; the 4 lanes of a block of 32 hold it together.  Every lane of the wavefront takes part (the
+// logarithm's table is exchanged between lanes).  Returns the block's scale byte.
+template <int FMT, int DT>
+__device__ __forceinline__ uint32_t encode8(const uint4& raw, const AppendParams& p, const WaveLog2& meta, uint32_t* w) {
+  using TR = DTypeTraits<DT>;
+  float x[8];
+  TR::unpack(raw, x);
+  uint32_t c[8];
+  uint32_t scale;
+  if constexpr (FMT == MASE_KV_MXINT8) {
+    const uint32_t m = group_max_u32<4>(vec_absmax_bits<DT>(raw));
+    int k = 0, kc = 0;
+    const int state = block_exponent<DT>(m, p.mxint, k, kc, meta);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float r = fminf(fmaxf(rintf(ldexpf(x[j], 7 - k)), -128.0f), 127.0f);
+      c[j] = state == 0 ? (uint32_t)(int)r & 0xFFu : 0u;
+    }
+    scale = state == 0 ? (uint32_t)(kc + 127) : 255u;  // the quantizer's other blocks are NaN throughout
+  } else {
+    constexpr int E = FMT == MASE_KV_MXFP8_E4M3 ? 4 : (FMT == MASE_KV_MXFP8_E5M2 ? 5 : 2), F = FMT == MASE_KV_MXFP8_E4M3 ? 3 : (FMT == MASE_KV_MXFP8_E5M2 ? 2 : 1);
+    const uint32_t m = group_max_u32<4>(vec_flushed_absmax<DT>(raw));
+    int sh = 0;
+    const int state = mxfp_block_scale(m, p.mxfp, sh, meta);
+    float y[8];
+    mxfp_elements<(E < 4), 8>(x, state, sh, p.mxfp, c, y);
+    uint32_t reserved = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) reserved |= code_is_reserved<E, F>(c[j]) ? 1u : 0u;
+    reserved = group_max_u32<4>(reserved);
+    int sb = state == 1 ? sh + 127 : (state == 0 ? 0 : 255);
+    if (state == 1 && reserved) {  // one scale up with halved codes, as the packing kernels write such blocks
+      sb = min(sb + 1, 254);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) c[j] = halve_code<E, F>(c[j]);
+    }
+    scale = (uint32_t)sb;
+  }
+  if constexpr (FMT == MASE_KV_MXFP4) {
+    w[0] = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[0] |= (c[j] & 0xFu) << (4 * j);
+  } else {
+    w[0] = c[0] | (c[1] << 8) | (c[2] << 16) | (c[3] << 24);
+    w[1] = c[4] | (c[5] << 8) | (c[6] << 16) | (c[7] << 24);
+  }
+  return scale;
+}
+
+// One 16-byte piece (8 elements) of keys and the same of values per lane; consecutive lanes go along the head dimension,
+// then the heads, then the tokens: the order in which projections leave their outputs.
+template <int D, int FMT, int DT>
+__global__ __launch_bounds__(256) void kv_append_kernel(AppendParams p) {
+  constexpr int kPieces = D / 8;
+  const int b = blockIdx.y;
+  const int count = p.counts == nullptr ? p.tokens : min(p.counts[b], p.tokens);
+  const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
+  const uint32_t first_token = (blockIdx.x * 256u) / kPieces / (uint32_t)p.c.heads;
+  if ((int)first_token >= count) return;  // the whole work-group
+  WaveLog2 meta;
+  if constexpr (FMT == MASE_KV_MXINT8) meta.init(p.mxint.tab, 0);
+  else if constexpr (FMT != MASE_KV_16BIT) meta.init(p.mxfp.tab, kLog2TabHalf);
+  const int piece = (int)(idx % kPieces);
+  const uint32_t r = idx / kPieces;
+  const int h = (int)(r % (uint32_t)p.c.heads), j = (int)(r / (uint32_t)p.c.heads);
+  int slot = -1, page = -1;
+  if (idx < p.items) {
+    slot = kv_new_slot(p.starts[b], count, j, p.c.table_pages, p.c.page_shift);
+    page = kv_page(p.c.table + (size_t)b * p.c.table_stride, p.c.table_pages, p.c.page_shift, p.c.num_pages, slot);
+  }
+  const bool live = page >= 0;
+  uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
+  if (live) {
+    kx = *(const uint4*)(p.key + (size_t)b * p.k_sb + (size_t)h * p.k_sh + (size_t)j * p.k_st + piece * 16);
+    vx = *(const uint4*)(p.value + (size_t)b * p.v_sb + (size_t)h * p.v_sh + (size_t)j * p.v_st + piece * 16);
+  }
+  const int row = slot & ((1 << p.c.page_shift) - 1);
+  const size_t ko = (size_t)page * p.c.k_page + (size_t)h * p.c.k_head + (size_t)row * p.c.k_slot;
+  const size_t vo = (size_t)page * p.c.v_page + (size_t)h * p.c.v_head + (size_t)row * p.c.v_slot;
+  if constexpr (FMT == MASE_KV_16BIT) {
+    if (!live) return;
+    *(uint4*)(p.c.k + ko + piece * 16) = kx;
+    *(uint4*)(p.c.v + vo + piece * 16) = vx;
+  } else {
+    uint32_t kw[2], vw[2];
+    const uint32_t ksb = encode8<FMT, DT>(kx, p, meta, kw), vsb = encode8<FMT, DT>(vx, p, meta, vw);
+    if (!live) return;
+    if constexpr (FMT == MASE_KV_MXFP4) {
+      *(uint32_t*)(p.c.k + ko + piece * 4) = kw[0];
+      *(uint32_t*)(p.c.v + vo + piece * 4) = vw[0];
+    } else {
+      *(uint2*)(p.c.k + ko + piece * 8) = make_uint2(kw[0], kw[1]);
+      *(uint2*)(p.c.v + vo + piece * 8) = make_uint2(vw[0], vw[1]);
+    }
+    if ((piece & 3) == 0) {
+      p.c.ks[key_scale_at<D>(p.c, page, h, row) + (piece >> 2)] = (uint8_t)ksb;
+      p.c.vs[value_scale_at<D>(p.c, page, h, row) + ((size_t)(piece >> 2) << p.c.page_shift)] = (uint8_t)vsb;
+    }
+  }
+  if (p.positions != nullptr && piece == 0)
+    p.positions[(size_t)b * p.pos_sb + (size_t)h * p.pos_sh + slot] =
+        (p.first_positions != nullptr ? p.first_positions[b] : p.starts[b]) + j;
+}
+
+template <int D, int FMT>
+void launch_append(const AppendParams& p, int dtype, size_t batch, hipStream_t st) {
+  const dim3 grid(blocks_for(p.items, 256), (unsigned)batch), block(256);
+  if (FMT == MASE_KV_16BIT || dtype == MASE_DT_BF16)
+    hipLaunchKernelGGL((kv_append_kernel<D, FMT, MASE_DT_BF16>), grid, block, 0, st, p);
+  else
+    hipLaunchKernelGGL((kv_append_kernel<D, FMT, MASE_DT_F16>), grid, block, 0, st, p);
+}
+
+// -------------------------------------------------------------------------------------------------
+// gather
+// -------------------------------------------------------------------------------------------------
+struct GatherParams {
+  PagedKv c;
+  const int32_t* lengths;
+  unsigned char* key;
+  unsigned char* value;
+  int max_length;
+};
+
+// 16 elements (codes) or 8 (16-bit rows) of keys and of values per lane
+template <int D, int FMT, bool F16>
+__global__ __launch_bounds__(256) void kv_gather_kernel(GatherParams p) {
+  constexpr int kE = FMT == MASE_KV_16BIT ? 8 : 16;
+  constexpr int kPieces = D / kE;
+  constexpr int kBytes = FMT == MASE_KV_16BIT ? 16 : (FMT == MASE_KV_MXFP4 ? 8 : 16);  // in storage
+  const int b = blockIdx.z, h = blockIdx.y;
+  const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
+  const int slot = (int)(idx / kPieces), piece = (int)(idx % kPieces);
+  if (slot >= p.max_length) return;
+  const int length = kv_length(p.lengths[b], p.max_length, p.c.table_pages, p.c.page_shift);
+  uint32_t kw[kE / 2], vw[kE / 2];
+#pragma unroll
+  for (int j = 0; j < kE / 2; ++j) kw[j] = vw[j] = 0;
+  const int page = slot < length ? kv_page(p.c.table + (size_t)b * p.c.table_stride, p.c.table_pages, p.c.page_shift, p.c.num_pages, slot) : -1;
+  if (page >= 0) {
+    const int row = slot & ((1 << p.c.page_shift) - 1);
+    uint32_t kc[kBytes / 4], vc[kBytes / 4];
+    kv_load<kBytes>(p.c.k + (size_t)page * p.c.k_page + (size_t)h * p.c.k_head + (size_t)row * p.c.k_slot + piece * kBytes, kc);
+    kv_load<kBytes>(p.c.v + (size_t)page * p.c.v_page + (size_t)h * p.c.v_head + (size_t)row * p.c.v_slot + piece * kBytes, vc);
+    float ks = 0.0f, vs = 0.0f;
+    if constexpr (FMT != MASE_KV_16BIT) {
+      ks = kv_scale<FMT>(p.c.ks[key_scale_at<D>(p.c, page, h, row) + piece / 2]);
+      vs = kv_scale<FMT>(p.c.vs[value_scale_at<D>(p.c, page, h, row) + ((size_t)(piece / 2) << p.c.page_shift)]);
+    }
+    kv_widen<FMT, F16, kE>(kc, ks, kw);
+    kv_widen<FMT, F16, kE>(vc, vs, vw);
+  }
+  const size_t at = ((((size_t)b * p.c.heads + h) * p.max_length + slot) * D + piece * kE) * 2;
+#pragma unroll
+  for (int j = 0; j < kE / 8; ++j) {
+    store_nt((uint4*)(p.key + at) + j, make_uint4(kw[4 * j], kw[4 * j + 1], kw[4 * j + 2], kw[4 * j + 3]));
+    store_nt((uint4*)(p.value + at) + j, make_uint4(vw[4 * j], vw[4 * j + 1], vw[4 * j + 2], vw[4 * j + 3]));
+  }
+}
+
+template <int D, int FMT>
+void launch_gather(const GatherParams& p, int dtype, size_t batch, hipStream_t st) {
+  constexpr int kPieces = D / (FMT == MASE_KV_16BIT ? 8 : 16);
+  const dim3 grid(blocks_for((size_t)p.max_length * kPieces, 256), (unsigned)p.c.heads, (unsigned)batch), block(256);
+  if (FMT == MASE_KV_16BIT || dtype == MASE_DT_BF16)
+    hipLaunchKernelGGL((kv_gather_kernel<D, FMT, false>), grid, block, 0, st, p);
+  else
+    hipLaunchKernelGGL((kv_gather_kernel<D, FMT, true>), grid, block, 0, st, p);
+}
+
+// -------------------------------------------------------------------------------------------------
+// evict
+// -------------------------------------------------------------------------------------------------
+struct EvictParams {
+  PagedKv c;
+  const int32_t* lengths;
+  const float* weights;
+  const int32_t* positions;
+  float* weights_out;
+  int32_t* positions_out;
+  int32_t* lengths_out;
+  int32_t* moves;    // [rows] number of moves (workspace)
+  int32_t* holes;    // [rows][keep] slots below keep that become free, in order
+  int32_t* fillers;  // [rows][keep] entry i: the i-th kept slot, for those at keep or behind
+  int max_length, capacity, keep, recent, first;
+};
+
+constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64;
+
+// a number that orders slots: protected ones above every weight, NaN below
+__device__ __forceinline__ uint32_t evict_key(float w, int pos, int newest, const EvictParams& p) {
+  if (pos < p.first || (long long)pos > (long long)newest - p.recent) return 0xFFFFFFFFu;
+  if (w != w) return 0u;
+  const uint32_t u = f2bits(w + 0.0f);  // -0 equals +0
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+__device__ __forceinline__ int lanes_below(uint64_t mask) {
+  return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
+}
+
+// One work-group per (sequence, cached head).  The key of the keep-th largest slot by three histogram passes over 11, 11
+// and 10 bits of the keys; then the kept slots in slot order, by counts per wavefront (a wavefront owns a contiguous run
+// of slots) and ballots within it.  Weights and positions are read once per pass, from L2 after the first.
+__global__ __launch_bounds__(kSelThreads) void kv_evict_select_kernel(EvictParams p) {
+  __shared__ uint32_t hist[2048];
+  __shared__ int sums[kSelWaves], sums2[kSelWaves];
+  __shared__ int sel_bin, sel_above;
+  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const size_t rowi = (size_t)b * p.c.heads + h;
+  const float* w = p.weights + rowi * p.capacity;
+  const int32_t* pos = p.positions + rowi * p.capacity;
+  float* wo = p.weights_out + rowi * p.capacity;
+  int32_t* po = p.positions_out + rowi * p.capacity;
+  const int n = kv_length(p.lengths[b], min(p.max_length, p.capacity), p.c.table_pages, p.c.page_shift);
+  if (h == 0 && tid == 0) p.lengths_out[b] = min(n, p.keep);
+  for (int s = min(n, p.keep) + tid; s < p.capacity; s += kSelThreads) {
+    wo[s] = 0.0f;
+    po[s] = -1;
+  }
+  if (n <= p.keep) {
+    for (int s = tid; s < n; s += kSelThreads) {
+      wo[s] = w[s];
+      po[s] = pos[s];
+    }
+    if (tid == 0) p.moves[rowi] = 0;
+    return;
+  }
+  // the largest position
+  int newest = -0x7FFFFFFF - 1;
+  for (int s = tid; s < n; s += kSelThreads) newest = max(newest, pos[s]);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) newest = max(newest, __shfl_xor(newest, d, 64));
+  if (lane == 0) sums[wave] = newest;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kSelWaves; ++i) newest = max(newest, sums[i]);
+
+  uint32_t prefix = 0, prefix_mask = 0;
+  int want = p.keep;  // how many of the slots that match the prefix are kept
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
+    const uint32_t bins = pass == 2 ? 1024u : 2048u;
+    hist[tid] = 0;
+    hist[tid + 1024] = 0;
+    __syncthreads();
+    for (int s0 = wave * 64; s0 < n; s0 += kSelThreads) {
+      const int s = s0 + lane;
+      const uint32_t key = s < n ? evict_key(w[s], pos[s], newest, p) : 0u;
+      const bool in = s < n && (key & prefix_mask) == prefix;
+      const uint32_t bin = (key >> shift) & (bins - 1);
+      // equal keys are common (tokens never attended to): those of the first lane's bin are added at once
+      const uint64_t act = __builtin_amdgcn_ballot_w64(in);
+      if (act != 0) {
+        const uint32_t lead = (uint32_t)__shfl((int)bin, (int)__builtin_ctzll(act), 64);
+        const uint64_t same = __builtin_amdgcn_ballot_w64(in && bin == lead);
+        if (in && bin != lead) atomicAdd(&hist[bin], 1u);
+        if (lane == 0) atomicAdd(&hist[lead], (uint32_t)__popcll(same));
+      }
+    }
+    __syncthreads();
+    // counts of the bins from the top: thread t has bins 2047 - 2t and 2046 - 2t
+    const int hi = (int)hist[2047 - 2 * tid], lo = (int)hist[2046 - 2 * tid];
+    int run = hi + lo;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(run, d, 64);
+      if (lane >= d) run += o;
+    }
+    if (lane == 63) sums[wave] = run;
+    __syncthreads();
+    int before = run - hi - lo;
+    for (int i = 0; i < wave; ++i) before += sums[i];
+    if (before < want && want <= before + hi + lo) {  // one thread: the kept ones end in one of its bins
+      const bool upper = want <= before + hi;
+      sel_bin = 2047 - 2 * tid - (upper ? 0 : 1);
+      sel_above = before + (upper ? 0 : hi);
+    }
+    __syncthreads();
+    want -= sel_above;
+    prefix |= (uint32_t)sel_bin << shift;
+    prefix_mask |= (bins - 1) << shift;
+    __syncthreads();
+  }
+  // keys above `prefix` are kept, and the first `want` that equal it
+  const int run_len = ((n + kSelThreads - 1) / kSelThreads) * 64;
+  const int s_lo = wave * run_len, s_hi = min(n, s_lo + run_len);
+  int gt = 0, eq = 0;
+  for (int s0 = s_lo; s0 < s_hi; s0 += 64) {
+    const int s = s0 + lane;
+    const uint32_t key = s < s_hi ? evict_key(w[s], pos[s], newest, p) : 0u;
+    gt += __popcll(__builtin_amdgcn_ballot_w64(s < s_hi && key > prefix));
+    eq += __popcll(__builtin_amdgcn_ballot_w64(s < s_hi && key == prefix));
+  }
+  if (lane == 0) {
+    sums[wave] = gt;
+    sums2[wave] = eq;
+  }
+  __syncthreads();
+  gt = 0;
+  eq = 0;
+  for (int i = 0; i < wave; ++i) {
+    gt += sums[i];
+    eq += sums2[i];
+  }
+  int32_t* holes = p.holes + rowi * p.keep;
+  int32_t* fillers = p.fillers + rowi * p.keep;
+  for (int s0 = s_lo; s0 < s_hi; s0 += 64) {
+    const int s = s0 + lane;
+    const bool in = s < s_hi;
+    const float wv = in ? w[s] : 0.0f;
+    const int pv = in ? pos[s] : 0;
+    const uint32_t key = evict_key(wv, pv, newest, p);
+    const uint64_t gm = __builtin_amdgcn_ballot_w64(in && key > prefix), em = __builtin_amdgcn_ballot_w64(in && key == prefix);
+    const int eq_before = eq + lanes_below(em);
+    const int kept_before = gt + lanes_below(gm) + min(eq_before, want);
+    const bool kept = in && (key > prefix || (key == prefix && eq_before < want));
+    if (in && s < p.keep) {
+      if (kept) {
+        wo[s] = wv;
+        po[s] = pv;
+      } else {
+        holes[s - kept_before] = s;
+      }
+    } else if (kept) {
+      fillers[kept_before] = s;  // kept_before < keep: exactly keep slots are kept
+    }
+    if (in && s == p.keep) p.moves[rowi] = p.keep - kept_before;
+    gt += __popcll(gm);
+    eq += __popcll(em);
+  }
+}
+
+// Moves kept rows from behind `keep` into the free slots: sources and targets are disjoint, so the order does not matter.
+// 16 bytes of keys and of values per lane.
+template <int D, int FMT>
+__global__ __launch_bounds__(256) void kv_evict_move_kernel(EvictParams p) {
+  constexpr int kRow = FMT == MASE_KV_16BIT ? 2 * D : (FMT == MASE_KV_MXFP4 ? D / 2 : D);
+  constexpr int kLanes = kRow / 16, kMoves = 256 / kLanes;
+  const int h = blockIdx.y, b = blockIdx.z;
+  const size_t rowi = (size_t)b * p.c.heads + h;
+  const int moves = p.moves[rowi];
+  const int part = threadIdx.x % kLanes;
+  const int32_t* table = p.c.table + (size_t)b * p.c.table_stride;
+  const int mask = (1 << p.c.page_shift) - 1;
+  for (int m = blockIdx.x * kMoves + (int)threadIdx.x / kLanes; m < moves; m += (int)gridDim.x * kMoves) {
+    const int to = p.holes[rowi * p.keep + m], from = p.fillers[rowi * p.keep + (p.keep - moves) + m];
+    if (part == 0) {
+      p.weights_out[rowi * p.capacity + to] = p.weights[rowi * p.capacity + from];
+      p.positions_out[rowi * p.capacity + to] = p.positions[rowi * p.capacity + from];
+    }
+    const int pf = kv_page(table, p.c.table_pages, p.c.page_shift, p.c.num_pages, from);
+    const int pt = kv_page(table, p.c.table_pages, p.c.page_shift, p.c.num_pages, to);
+    if (pf < 0 || pt < 0) continue;
+    const int rf = from & mask, rt = to & mask;
+    const size_t hk = (size_t)h * p.c.k_head + part * 16, hv = (size_t)h * p.c.v_head + part * 16;
+    const uint4 kx = *(const uint4*)(p.c.k + (size_t)pf * p.c.k_page + (size_t)rf * p.c.k_slot + hk);
+    const uint4 vx = *(const uint4*)(p.c.v + (size_t)pf * p.c.v_page + (size_t)rf * p.c.v_slot + hv);
+    *(uint4*)(p.c.k + (size_t)pt * p.c.k_page + (size_t)rt * p.c.k_slot + hk) = kx;
+    *(uint4*)(p.c.v + (size_t)pt * p.c.v_page + (size_t)rt * p.c.v_slot + hv) = vx;
+    if constexpr (FMT != MASE_KV_16BIT) {
+      if (part < D / 32) {
+        p.c.ks[key_scale_at<D>(p.c, pt, h, rt) + part] = p.c.ks[key_scale_at<D>(p.c, pf, h, rf) + part];
+        const size_t col = (size_t)part << p.c.page_shift;
+        p.c.vs[value_scale_at<D>(p.c, pt, h, rt) + col] = p.c.vs[value_scale_at<D>(p.c, pf, h, rf) + col];
+      }
+    }
+  }
+}
+
+template <int D, int FMT>
+void launch_evict_move(const EvictParams& p, size_t batch, hipStream_t st) {
+  constexpr int kLanes = (FMT == MASE_KV_16BIT ? 2 * D : (FMT == MASE_KV_MXFP4 ? D / 2 : D)) / 16;
+  const int most = min(p.keep, p.max_length - p.keep);  // of moves in a row
+  const dim3 grid(blocks_for((size_t)most, 256 / kLanes), (unsigned)p.c.heads, (unsigned)batch);
+  hipLaunchKernelGGL((kv_evict_move_kernel<D, FMT>), grid, dim3(256), 0, st, p);
+}
+
+// calls F<D, FMT>::run(args...) for the pool's head dimension and format
+#define MASE_KV_DISPATCH(cache, fn, ...)                                               \
+  do {                                                                                 \
+    switch ((int)(cache)->head_dim * 8 + (cache)->format) {                            \
+      MASE_KV_CASES(64, fn, __VA_ARGS__)                                               \
+      MASE_KV_CASES(128, fn, __VA_ARGS__)                                              \
+      MASE_KV_CASES(256, fn, __VA_ARGS__)                                              \
+      default: return MASE_ERR_SHAPE;                                                  \
+    }                                                                                  \
+  } while (0)
+#define MASE_KV_CASES(D, fn, ...)                                                      \
+  case D * 8 + MASE_KV_16BIT: fn<D, MASE_KV_16BIT>(__VA_ARGS__); break;                \
+  case D * 8 + MASE_KV_MXINT8: fn<D, MASE_KV_MXINT8>(__VA_ARGS__); break;              \
+  case D * 8 + MASE_KV_MXFP8_E4M3: fn<D, MASE_KV_MXFP8_E4M3>(__VA_ARGS__); break;      \
+  case D * 8 + MASE_KV_MXFP8_E5M2: fn<D, MASE_KV_MXFP8_E5M2>(__VA_ARGS__); break;      \
+  case D * 8 + MASE_KV_MXFP4: fn<D, MASE_KV_MXFP4>(__VA_ARGS__); break;
+
+MxfpParams mxfp_params(int format, const uint32_t* tab) {
+  MxfpParams q{};
+  q.m.E = format == MASE_KV_MXFP8_E4M3 ? 4 : (format == MASE_KV_MXFP8_E5M2 ? 5 : 2);
+  q.m.F = format == MASE_KV_MXFP8_E4M3 ? 3 : (format == MASE_KV_MXFP8_E5M2 ? 2 : 1);
+  q.m.bias = (1 << (q.m.E - 1)) - 1;
+  q.m.e_hi = (1 << q.m.E) - 1;
+  q.m.frac_hi = (1 << q.m.F) - 1;
+  q.m.is_finite = 1;
+  q.m.round_mode = 0;
+  q.el_emax = q.m.e_hi - q.m.bias;
+  q.tab = tab;
+  return q;
+}
+
+}  // namespace
+}  // namespace mase
+
+extern "C" int mase_paged_kv_append(const mase_paged_kv* cache, const void* key, const void* value, size_t tokens,
+                                    size_t key_stride_b, size_t key_stride_h, size_t key_stride_t, size_t value_stride_b,
+                                    size_t value_stride_h, size_t value_stride_t, const int32_t* starts,
+                                    const int32_t* counts, int32_t* positions, size_t pos_stride_b, size_t pos_stride_h,
+                                    const int32_t* first_positions, const uint32_t* log2_tab, void* stream) {
+  using namespace mase;
+  AppendParams p{};
+  const int rc = paged_kv_params(cache, p.c);
+  if (rc != MASE_OK) return rc;
+  if (cache->batch == 0 || tokens == 0) return MASE_OK;
+  if (key == nullptr || value == nullptr || starts == nullptr) return MASE_ERR_NULL;
+  if (cache->format != MASE_KV_16BIT && log2_tab == nullptr) return MASE_ERR_NULL;
+  if (!aligned16(key) || !aligned16(value)) return MASE_ERR_ALIGN;
+  const size_t strides[6] = {key_stride_b, key_stride_h, key_stride_t, value_stride_b, value_stride_h, value_stride_t};
+  for (size_t s : strides)
+    if (s % 8 != 0) return MASE_ERR_ALIGN;
+  if (tokens > 0x7FFFFF00u / (cache->kv_heads * (cache->head_dim / 8))) return MASE_ERR_SHAPE;
+  p.key = (const unsigned char*)key;
+  p.value = (const unsigned char*)value;
+  p.k_sb = key_stride_b * 2; p.k_sh = key_stride_h * 2; p.k_st = key_stride_t * 2;
+  p.v_sb = value_stride_b * 2; p.v_sh = value_stride_h * 2; p.v_st = value_stride_t * 2;
+  p.starts = starts;
+  p.counts = counts;
+  p.positions = positions;
+  p.pos_sb = pos_stride_b;
+  p.pos_sh = pos_stride_h;
+  p.first_positions = first_positions;
+  p.tokens = (int)tokens;
+  p.items = (uint32_t)(tokens * cache->kv_heads * (cache->head_dim / 8));
+  if (cache->format == MASE_KV_MXINT8) {
+    p.mxint.qshift = 7;
+    p.mxint.bias = 127;
+    p.mxint.scale_max = 255;
+    p.mxint.lo = -128.0f;
+    p.mxint.hi = 127.0f;
+    p.mxint.tab = log2_tab;
+  } else if (cache->format != MASE_KV_16BIT) {
+    p.mxfp = mxfp_params(cache->format, log2_tab);
+  }
+  MASE_KV_DISPATCH(cache, launch_append, p, cache->dtype, cache->batch, (hipStream_t)stream);
+  return hipGetLastError() == hipSuccess ? MASE_OK : MASE_ERR_LAUNCH;
+}
+
+extern "C" int mase_paged_kv_gather(const mase_paged_kv* cache, const int32_t* lengths, size_t max_length, void* key,
+                                    void* value, void* stream) {
+  using namespace mase;
+  GatherParams p{};
+  const int rc = paged_kv_params(cache, p.c);
+  if (rc != MASE_OK) return rc;
+  if (cache->batch == 0 || max_length == 0) return MASE_OK;
+  if (lengths == nullptr || key == nullptr || value == nullptr) return MASE_ERR_NULL;
+  if (!aligned16(key) || !aligned16(value)) return MASE_ERR_ALIGN;
+  if (max_length > 0x7FFFFF00u / (cache->head_dim / 8)) return MASE_ERR_SHAPE;
+  p.lengths = lengths;
+  p.key = (unsigned char*)key;
+  p.value = (unsigned char*)value;
+  p.max_length = (int)max_length;
+  MASE_KV_DISPATCH(cache, launch_gather, p, cache->dtype, cache->batch, (hipStream_t)stream);
+  return hipGetLastError() == hipSuccess ? MASE_OK : MASE_ERR_LAUNCH;
+}
+
+extern "C" size_t mase_paged_kv_evict_workspace_bytes(size_t batch, size_t kv_heads, size_t keep) {
+  const size_t rows = batch * kv_heads;
+  return ((rows + 3) / 4 * 4 + 2 * rows * keep) * sizeof(int32_t);
+}
+
+extern "C" int mase_paged_kv_evict(const mase_paged_kv* cache, const int32_t* lengths, size_t max_length,
+                                   const float* weights, const int32_t* positions, size_t capacity, size_t keep,
+                                   size_t recent, size_t first, float* weights_out, int32_t* positions_out,
+                                   int32_t* lengths_out, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace mase;
+  EvictParams p{};
+  const int rc = paged_kv_params(cache, p.c);
+  if (rc != MASE_OK) return rc;
+  if (keep == 0 || recent > keep || first > keep - recent) return MASE_ERR_PARAM;
+  if (cache->batch == 0) return MASE_OK;
+  if (lengths == nullptr || weights == nullptr || positions == nullptr || weights_out == nullptr ||
+      positions_out == nullptr || lengths_out == nullptr)
+    return MASE_ERR_NULL;
+  if (weights == weights_out || positions == positions_out) return MASE_ERR_PARAM;
+  if (max_length > 0x7FFFFFFFu - 1024u || capacity == 0 || capacity > 0x7FFFFFFFu - 1024u || keep > 0x7FFFFFFFu) return MASE_ERR_SHAPE;
+  const size_t rows = cache->batch * cache->kv_heads;
+  if (workspace == nullptr || workspace_bytes < mase_paged_kv_evict_workspace_bytes(cache->batch, cache->kv_heads, keep))
+    return MASE_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return MASE_ERR_ALIGN;
+  p.lengths = lengths;
+  p.weights = weights;
+  p.positions = positions;
+  p.weights_out = weights_out;
+  p.positions_out = positions_out;
+  p.lengths_out = lengths_out;
+  p.moves = (int32_t*)workspace;
+  p.holes = p.moves + (rows + 3) / 4 * 4;
+  p.fillers = p.holes + rows * keep;
+  p.max_length = (int)max_length;
+  p.capacity = (int)capacity;
+  p.keep = (int)keep;
+  p.recent = (int)recent;
+  p.first = (int)first;
+  hipStream_t st = (hipStream_t)stream;
+  hipLaunchKernelGGL(kv_evict_select_kernel, dim3((unsigned)cache->kv_heads, (unsigned)cache->batch), dim3(kSelThreads), 0,
+                     st, p);
+  if (max_length > keep && capacity > keep) MASE_KV_DISPATCH(cache, launch_evict_move, p, cache->batch, st);
+  return hipGetLastError() == hipSuccess ? MASE_OK : MASE_ERR_LAUNCH;
+}

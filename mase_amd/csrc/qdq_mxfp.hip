@@ -20,13 +20,6 @@ namespace {
 
 constexpr int kVecThreads = 64;
 
-// largest magnitude (fp32 bits) of the flushed elements of one 16-byte input vector
-template <int DTI>
-__device__ __forceinline__ uint32_t vec_flushed_absmax(const uint4& v) {
-  const uint32_t m = vec_absmax_bits<DTI>(v);
-  return ((m & 0x7F800000u) == 0) ? 0u : m;  // a subnormal maximum means every element is flushed
-}
-
 // One 16-byte vector of the wider side per lane, 64-lane work-groups (the shape that streams best on this
 // part); a block of B elements spans LPB lanes, or a lane holds SUB blocks.  No lane leaves before the table
 // lookups: they are wave-wide register permutes.
@@ -286,31 +279,6 @@ int launch_mxfp(const void* in, void* out, uint8_t* codes, uint8_t* scales, size
 // subnormal range below that (error <= 2^-10 of an element unit while the block maximum is >= 2^8 units).
 // 8-bit codes are stored one per byte, 4-bit codes two per byte (even element in the low nibble).
 // ---------------------------------------------------------------------------------------------
-template <int E, int F>
-__device__ __forceinline__ uint32_t halve_code(uint32_t c) {
-  const uint32_t sgn = c & (1u << (E + F));
-  uint32_t e = (c >> F) & ((1u << E) - 1u);
-  uint32_t f = c & ((1u << F) - 1u);
-  if (e >= 2) {
-    e -= 1;
-  } else {
-    uint32_t v = (e == 1) ? ((1u << F) + f) : f;
-    uint32_t q = (v >> 1) + ((v & 1u) & ((v >> 1) & 1u));  // round half to even
-    if (q == (1u << F)) { e = 1; f = 0; }
-    else { e = 0; f = q; }
-  }
-  return sgn | (e << F) | f;
-}
-
-template <int E, int F>
-__device__ __forceinline__ bool code_is_reserved(uint32_t c) {
-  const uint32_t e = (c >> F) & ((1u << E) - 1u);
-  const uint32_t f = c & ((1u << F) - 1u);
-  if constexpr (E == 4 && F == 3) return e == 15u && f == 7u;  // OCP e4m3: NaN
-  if constexpr (E == 5 && F == 2) return e == 31u;             // OCP e5m2: Inf / NaN
-  return false;
-}
-
 // TILED (8-bit codes only): the codes of a [rows, K] matrix go to the image the tiled block-scaled GEMM copies from,
 // [row tile of 256][K tile of 128][row][128 B] with the 16-byte chunks of a row segment exchanged by
 // chunk ^= (row >> 1) & 7 (the GEMM's LDS swizzle); k8 = K / 8 lanes per row.  Scales stay row-major.

@@ -14,3 +14,4 @@ from .activations import (  # noqa: F401
     softmax_mxfp,
     softmax_mxint,
 )
+from .paged_kv import paged_attention_decode, paged_kv_append, paged_kv_evict, paged_kv_gather  # noqa: F401

@@ -12,10 +12,13 @@ matrix-core kernel of this package for bf16 operands (``mase_gemm_bf16_tn_batche
 
 What is quantized (``q_config`` sub-dicts, each with an optional ``bypass``):
   ``rope``      cos/sin tables, minifloat cast                       (attention.py:163-177)
-  ``kv_cache``  new key/value states before ``past_key_value.update``  (attention.py:182-187)
+  ``kv_cache``  new key/value states before ``past_key_value.update``  (attention.py:182-187); a ``PagedKVCache`` with
+                codes of the same format quantizes as it writes
   ``qk_matmul`` the query (not the key) along head_dim                (attention.py:352-361)
   ``softmax``   the masked scores, minifloat cast, softmax in fp32    (attention.py:369-375)
   ``av_matmul`` the probabilities (not the values) along the key axis (attention.py:383-392)
+With a ``PagedKVCache`` as ``past_key_value``, a step of one new token with ``softmax`` and ``av_matmul`` bypassed is
+attended from the pages (no attention weights are returned); other steps read the cache back dense.
 MLP: ``silu_minifloat`` on the gate projection (mlp.py:60-62, 75-77); RMSNorm: minifloat cast of the input and of the
 weight (rms_norm.py:72-84).
 """
@@ -31,6 +34,7 @@ from ..._gemm import matmul_bf16
 from ...quantizers import mxfp_quantizer, mxint_quantizer
 from ...quantizers import _ops
 from ...quantizers._ops import attn_softmax_mx, attn_softmax_mx_supported, minifloat_mx_qdq
+from ..paged_cache import PagedKVCache
 from ..functional.mx_linear import project_shared
 from ..functional.activations import kv_cache_mxfp, kv_cache_mxint, rope_minifloat, rotate_half, silu_minifloat, softmax_minifloat
 
@@ -182,7 +186,13 @@ class _LlamaAttentionMX(nn.Module):
 
         if past_key_value is not None:
             cache_kwargs = {"sin": sin, "cos": cos, "cache_position": cache_position}
-            if not self.kv_cache_bypass:
+            paged = isinstance(past_key_value, PagedKVCache)
+            if paged:
+                past_key_value.require_kind(None if self.kv_cache_bypass else self._kind, self.kv_cache_config)
+                if self._reads_pages(query_states, attention_mask):
+                    return self._attend_pages(past_key_value, query_states, key_states, value_states, attention_mask, input_shape)
+            # a packed paged cache quantizes what it writes
+            if not self.kv_cache_bypass and not (paged and past_key_value.kv_format is not None):
                 kv_cache = kv_cache_mxfp if self._kind == "mxfp" else kv_cache_mxint
                 key_states, value_states = kv_cache(key_states, value_states, self.kv_cache_config)
             key_states, value_states = past_key_value.update(key_states, value_states, self.layer_idx, cache_kwargs)
@@ -195,6 +205,23 @@ class _LlamaAttentionMX(nn.Module):
         attn_output = attn_output.reshape(*input_shape, -1).contiguous()
         attn_output = self.o_proj(attn_output)
         return attn_output, attn_weights
+
+    def _reads_pages(self, query_states, attention_mask):
+        """whether this step is one new token whose attention needs nothing between scores and values but the softmax:
+        then it is computed from the pages of a ``PagedKVCache``; otherwise the cache is read back dense"""
+        if query_states.shape[2] != 1 or not (self.softmax_bypass and self.av_bypass):
+            return False
+        if self.training and self.attention_dropout != 0.0 or (torch.is_grad_enabled() and query_states.requires_grad):
+            return False
+        return attention_mask is None or (attention_mask.dim() == 4 and tuple(attention_mask.shape[1:3]) == (1, 1)
+                                          and attention_mask.dtype in (query_states.dtype, torch.float32))
+
+    def _attend_pages(self, cache, query_states, key_states, value_states, attention_mask, input_shape):
+        cache.append(key_states, value_states, self.layer_idx)
+        if not self.qk_bypass:
+            query_states = _mx_quantizer(self._kind, self.qk_config)(query_states)
+        out = cache.attend(query_states[:, :, 0], self.layer_idx, scaling=self.scaling, mask=attention_mask)
+        return self.o_proj(out.reshape(*input_shape, -1)), None
 
     def _project(self, hidden_states, hidden_shape):
         """query / key / value states [batch, heads, seq, head_dim] (attention.py:157-159)"""

@@ -1,0 +1,210 @@
+"""``PagedKVCache``: the keys and values of a batch of sequences in pages, as 16-bit states or as MX codes.
+
+It takes the place of the cache object that the attention modules call ``past_key_value.update`` on
+(``chop/nn/quantized/modules/llama/attention.py:182-187``): ``update`` appends and returns the dense states, ``append`` and
+``attend`` do a decoding step on the pages alone, and ``evict`` cuts the sequences down to a budget by the attention
+weights that ``attend`` has added up.  The functions underneath are in ``mase_amd.quantized.functional``.
+
+The host keeps how long each sequence is, so no call waits for the GPU; a step that is captured into a graph uses the
+functions directly, with lengths that the graph itself moves on.
+"""
+from __future__ import annotations
+
+from typing import List, Optional, Sequence, Tuple
+
+import torch
+from torch import Tensor
+
+from .functional import paged_kv as F
+
+# (kind, element bits or exponent and fraction bits) of the kv_cache quantizer that each code format holds the values of
+_FORMAT_OF = {("mxint", 8): "mxint8", ("mxfp", 4, 3): "mxfp8_e4m3", ("mxfp", 5, 2): "mxfp8_e5m2", ("mxfp", 2, 1): "mxfp4"}
+
+
+class PagedKVCache:
+    """``batch_size`` sequences of at most ``max_length`` tokens at a time, ``num_layers`` layers that share one page table.
+
+    ``kv_format``: None (states of ``dtype``), ``"mxint8"``, ``"mxfp8_e4m3"``, ``"mxfp8_e5m2"`` or ``"mxfp4"`` (blocks of 32
+    along the head dimension).  ``num_pages`` (default: enough for every sequence at ``max_length``) is the pool's size for
+    each layer; a sequence takes pages as it grows.  ``track_weights``: ``attend`` adds up the attention weights and
+    positions are kept, which ``evict`` needs."""
+
+    def __init__(self, batch_size: int, num_kv_heads: int, head_dim: int, max_length: int, num_layers: int = 1, *,
+                 page_size: int = 64, num_pages: Optional[int] = None, kv_format: Optional[str] = None,
+                 dtype: torch.dtype = torch.bfloat16, device="cuda", track_weights: bool = False):
+        if kv_format not in F.KV_FORMATS:
+            raise ValueError(f"kv_format must be one of {F.KV_FORMATS}, got {kv_format!r}")
+        if min(batch_size, num_kv_heads, max_length, num_layers) < 1:
+            raise ValueError("batch_size, num_kv_heads, max_length and num_layers must be at least 1")
+        if head_dim not in (64, 128, 256) or page_size not in (16 << n for n in range(9)):
+            raise ValueError(f"head_dim must be 64, 128 or 256 and page_size a power of two from 16 to 4096, got {head_dim} and {page_size}")
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"dtype must be bfloat16 or float16, got {dtype}")
+        self.batch_size, self.num_kv_heads, self.head_dim, self.max_length = batch_size, num_kv_heads, head_dim, max_length
+        self.num_layers, self.page_size, self.kv_format, self.dtype = num_layers, page_size, kv_format, dtype
+        self.device = torch.device(device)
+        table_pages = -(-max_length // page_size)
+        self.num_pages = batch_size * table_pages if num_pages is None else int(num_pages)
+        if self.num_pages < 1:
+            raise ValueError("num_pages must be at least 1")
+        shape = (num_layers, self.num_pages, num_kv_heads, page_size)
+        if kv_format is None:
+            self._k, self._v = (torch.zeros((*shape, head_dim), dtype=dtype, device=self.device) for _ in range(2))
+            self._ks = self._vs = None
+        else:
+            width = head_dim // 2 if kv_format == "mxfp4" else head_dim
+            code = torch.int8 if kv_format == "mxint8" else torch.uint8
+            self._k, self._v = (torch.zeros((*shape, width), dtype=code, device=self.device) for _ in range(2))
+            self._ks = torch.zeros((*shape, head_dim // 32), dtype=torch.uint8, device=self.device)
+            self._vs = torch.zeros((*shape[:3], head_dim // 32, page_size), dtype=torch.uint8, device=self.device)
+        self._table = torch.full((batch_size, table_pages), -1, dtype=torch.int32, device=self.device)
+        self._free = list(range(self.num_pages - 1, -1, -1))
+        self._pages: List[List[int]] = [[] for _ in range(batch_size)]
+        # per layer: slots held and tokens seen, on the host and on the device
+        self._held = [[0] * batch_size for _ in range(num_layers)]
+        self._seen = [[0] * batch_size for _ in range(num_layers)]
+        self._held_dev, self._seen_dev = (torch.zeros((num_layers, batch_size), dtype=torch.int32, device=self.device) for _ in range(2))
+        self.track_weights = track_weights
+        self._weights = self._positions = None
+        if track_weights:
+            rows = (num_layers, batch_size, num_kv_heads, table_pages * page_size)
+            self._weights = torch.zeros(rows, dtype=torch.float32, device=self.device)
+            self._positions = torch.full(rows, -1, dtype=torch.int32, device=self.device)
+
+    # -- what it holds ------------------------------------------------------------------------------------------------
+    def get_seq_length(self, layer_idx: int = 0) -> int:
+        """tokens that the longest sequence has seen: the position of the next one"""
+        return max(self._seen[layer_idx])
+
+    def lengths(self, layer_idx: int = 0) -> List[int]:
+        """slots that each sequence holds (fewer than it has seen after an eviction)"""
+        return list(self._held[layer_idx])
+
+    def positions(self, layer_idx: int = 0) -> Tensor:
+        """int32 ``[batch, kv_heads, capacity]``: where the token of each slot stood, -1 for free slots"""
+        self._require_tracking("positions")
+        return self._positions[layer_idx]
+
+    def weights(self, layer_idx: int = 0) -> Tensor:
+        """float32 ``[batch, kv_heads, capacity]``: attention weights added up by ``attend``"""
+        self._require_tracking("weights")
+        return self._weights[layer_idx]
+
+    def require_kind(self, kind: Optional[str], config: dict) -> None:
+        """raises ValueError unless states quantized by the module's ``kv_cache`` configuration (``kind`` None: not
+        quantized) are what this cache holds: codes hold the values of one quantizer only, 16-bit pages those of any"""
+        if self.kv_format is None:
+            return
+        if kind is None:
+            raise ValueError(f"a PagedKVCache of {self.kv_format} codes quantizes what it holds, but the module's kv_cache quantizer is bypassed: use kv_format=None")
+        bits = (config["data_in_width"],) if kind == "mxint" else (config["data_in_exponent_width"], config["data_in_frac_width"])
+        if config["data_in_block_size"] != 32 or _FORMAT_OF.get((kind, *bits)) != self.kv_format:
+            raise ValueError(f"a PagedKVCache of {self.kv_format} codes does not hold the values of the module's kv_cache quantizer ({kind}, {config}): use kv_format=None")
+
+    # -- a step -------------------------------------------------------------------------------------------------------
+    def append(self, key_states: Tensor, value_states: Tensor, layer_idx: int = 0, counts: Optional[Sequence[int]] = None) -> None:
+        """adds ``[batch, kv_heads, tokens, head_dim]`` states behind what the layer holds; ``counts[b]`` of the tokens for
+        sequence b where given (a padded batch)"""
+        if key_states.dim() != 4 or key_states.shape[0] != self.batch_size or key_states.dtype != self.dtype:
+            raise ValueError(f"states must be {self.dtype} [{self.batch_size}, {self.num_kv_heads}, tokens, {self.head_dim}], got {key_states.dtype} {tuple(key_states.shape)}")
+        n = key_states.shape[2]
+        new = [n] * self.batch_size if counts is None else [int(c) for c in counts]
+        if len(new) != self.batch_size or any(c < 0 or c > n for c in new):
+            raise ValueError(f"counts must be {self.batch_size} numbers from 0 to {n}, got {new}")
+        held, seen = self._held[layer_idx], self._seen[layer_idx]
+        self._grow([h + c for h, c in zip(held, new)])
+        counts_dev = None if counts is None else torch.tensor(new, dtype=torch.int32, device=self.device)
+        track = dict(positions=self._positions[layer_idx], first_positions=self._seen_dev[layer_idx]) if self.track_weights else {}
+        F.paged_kv_append(key_states, value_states, *self._pool(layer_idx), self._held_dev[layer_idx], counts=counts_dev, **track,
+                          **self._codes(layer_idx))
+        for b, c in enumerate(new):
+            held[b] += c
+            seen[b] += c
+        step = n if counts_dev is None else counts_dev
+        self._held_dev[layer_idx] += step
+        self._seen_dev[layer_idx] += step
+
+    def update(self, key_states: Tensor, value_states: Tensor, layer_idx: int = 0, cache_kwargs=None) -> Tuple[Tensor, Tensor]:
+        """appends, and returns all that the layer holds as ``[batch, kv_heads, longest, head_dim]``, zeros behind shorter
+        sequences"""
+        self.append(key_states, value_states, layer_idx)
+        return self.gather(layer_idx)
+
+    def gather(self, layer_idx: int = 0) -> Tuple[Tensor, Tensor]:
+        return F.paged_kv_gather(*self._pool(layer_idx), self._held_dev[layer_idx], max(self._held[layer_idx]), dtype=self.dtype,
+                                 **self._codes(layer_idx))
+
+    def attend(self, query: Tensor, layer_idx: int = 0, *, scaling: Optional[float] = None, mask: Optional[Tensor] = None) -> Tensor:
+        """attention of one token per sequence, ``[batch, heads, head_dim]``, over what the layer holds"""
+        return F.paged_attention_decode(query, *self._pool(layer_idx), self._held_dev[layer_idx], max(self._held[layer_idx]),
+                                        scaling=scaling, mask=mask, weights=self._weights[layer_idx] if self.track_weights else None,
+                                        **self._codes(layer_idx))
+
+    # -- room ---------------------------------------------------------------------------------------------------------
+    def evict(self, keep: int, *, recent: int = 0, first: int = 0) -> None:
+        """cuts every sequence down to ``keep`` tokens in every layer and cached head (see ``paged_kv_evict``) and gives the
+        pages behind them back; between steps, when all layers hold the same tokens"""
+        self._require_tracking("evict")
+        if any(h != self._held[0] for h in self._held):
+            raise ValueError("evict() comes between steps: the layers do not hold the same number of tokens")
+        longest = max(self._held[0])
+        if longest <= keep:
+            return
+        for layer in range(self.num_layers):
+            w, pos, n = F.paged_kv_evict(*self._pool(layer), self._held_dev[layer], self._weights[layer], self._positions[layer],
+                                         longest, keep, recent=recent, first=first, **self._codes(layer))
+            self._weights[layer].copy_(w)
+            self._positions[layer].copy_(pos)
+            self._held_dev[layer].copy_(n)
+            self._held[layer] = [min(h, keep) for h in self._held[layer]]
+        dropped = []
+        for b, pages in enumerate(self._pages):
+            left = -(-self._held[0][b] // self.page_size)
+            dropped += [(b, i) for i in range(left, len(pages))]
+            self._free += reversed(pages[left:])
+            del pages[left:]
+        self._set_table(dropped, [-1] * len(dropped))
+
+    def reset(self) -> None:
+        """forgets every sequence"""
+        self._free = list(range(self.num_pages - 1, -1, -1))
+        self._pages = [[] for _ in range(self.batch_size)]
+        self._held, self._seen = ([[0] * self.batch_size for _ in range(self.num_layers)] for _ in range(2))
+        for t in (self._held_dev, self._seen_dev) + ((self._weights,) if self.track_weights else ()):
+            t.zero_()
+        self._table.fill_(-1)
+        if self.track_weights:
+            self._positions.fill_(-1)
+
+    # -- inside -------------------------------------------------------------------------------------------------------
+    def _require_tracking(self, what: str) -> None:
+        if not self.track_weights:
+            raise ValueError(f"{what} needs a cache made with track_weights=True")
+
+    def _pool(self, layer: int):
+        return self._k[layer], self._v[layer], self._table
+
+    def _codes(self, layer: int) -> dict:
+        if self.kv_format is None:
+            return {}
+        return dict(kv_format=self.kv_format, k_scales=self._ks[layer], v_scales=self._vs[layer])
+
+    def _grow(self, lengths: Sequence[int]) -> None:
+        """pages for sequences of these lengths"""
+        if max(lengths) > self.max_length:
+            raise ValueError(f"a sequence of {max(lengths)} tokens does not fit a cache of max_length {self.max_length}")
+        need = [max(0, -(-n // self.page_size) - len(p)) for n, p in zip(lengths, self._pages)]
+        if sum(need) > len(self._free):
+            raise ValueError(f"the pool has {len(self._free)} free pages, {sum(need)} are needed")
+        at, got = [], []
+        for b, k in enumerate(need):
+            for _ in range(k):
+                at.append((b, len(self._pages[b])))
+                got.append(self._free.pop())
+                self._pages[b].append(got[-1])
+        self._set_table(at, got)
+
+    def _set_table(self, at, pages) -> None:
+        if at:
+            rows, cols = torch.tensor(at, device=self.device).unbind(1)
+            self._table[rows, cols] = torch.tensor(pages, dtype=torch.int32, device=self.device)
