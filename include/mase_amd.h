@@ -476,9 +476,9 @@ int mase_paged_kv_gather(const mase_paged_kv* cache, const int32_t* lengths, siz
  * weights (optional, fp32) [batch][kv_heads][...] by element strides of batch and head: entry t grows by the probabilities
  * of slot t summed over the query heads of its cached head, in a fixed order.
  * The cache is split over its length; the parts (and with weights the scores) pass through `workspace`,
- * mase_paged_attention_decode_workspace_bytes() bytes, 16-byte aligned (0 bytes: NULL will do). */
+ * mase_paged_attention_decode_workspace_bytes() bytes, 16-byte aligned (0: no such call). */
 size_t mase_paged_attention_decode_workspace_bytes(size_t batch, size_t heads, size_t kv_heads, size_t head_dim,
-                                                   size_t max_length, int with_weights);
+                                                   int format, size_t max_length, int with_weights);
 int mase_paged_attention_decode(const mase_paged_kv* cache, const void* q, size_t q_stride_b, size_t q_stride_h, size_t heads,
                                 const int32_t* lengths, size_t max_length, float scaling, const void* mask, int mask_dtype,
                                 size_t mask_stride_b, float* weights, size_t w_stride_b, size_t w_stride_h, void* out,

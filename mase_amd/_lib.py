@@ -101,7 +101,7 @@ SIGNATURES = {
     "mase_paged_kv_append": (c_int, [c_void_p, c_void_p, c_void_p] + [c_size_t] * 7 + [c_void_p, c_void_p, c_void_p, c_size_t, c_size_t,
                                      c_void_p, c_void_p, c_void_p]),
     "mase_paged_kv_gather": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p, c_void_p, c_void_p]),
-    "mase_paged_attention_decode_workspace_bytes": (c_size_t, [c_size_t] * 5 + [c_int]),
+    "mase_paged_attention_decode_workspace_bytes": (c_size_t, [c_size_t] * 4 + [c_int, c_size_t, c_int]),
     "mase_paged_attention_decode": (c_int, [c_void_p, c_void_p, c_size_t, c_size_t, c_size_t, c_void_p, c_size_t, c_float, c_void_p,
                                             c_int, c_size_t, c_void_p, c_size_t, c_size_t, c_void_p, c_void_p, c_size_t, c_void_p]),
     "mase_paged_kv_evict_workspace_bytes": (c_size_t, [c_size_t] * 3),

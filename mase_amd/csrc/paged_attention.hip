@@ -14,6 +14,18 @@
 // MX codes are widened to 16 bits in registers as they are used (exact), two per conversion instruction for MXFP.
 #include "paged_kv.hpp"
 
+#ifndef MASE_PA_U8
+#define MASE_PA_U8 1
+#endif
+#ifndef MASE_PA_U4
+#define MASE_PA_U4 1
+#endif
+#ifndef MASE_PA_OCC
+#define MASE_PA_OCC 3
+#endif
+#ifndef MASE_PA_ROUNDS
+#define MASE_PA_ROUNDS 1
+#endif
 namespace mase {
 namespace {
 
@@ -22,8 +34,6 @@ typedef _Float16 pa_f16x8_t __attribute__((ext_vector_type(8)));
 typedef float pa_f32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;
-constexpr int kSlots = 32;                  // per wavefront and step
-constexpr int kChunkStep = kWaves * kSlots;  // lengths of parts are multiples of it
 constexpr int kHeadTile = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -36,13 +46,15 @@ struct DecodeParams {
   size_t mask_sb;  // elements
   int mask_f32;
   unsigned char* out;
-  float* part_o;   // [batch * heads][splits][D]
-  float* part_ml;  // [batch * heads][splits][2]
-  float* scores;   // [batch * heads][score_stride], NULL without weights
+  unsigned long long* plan;  // [batch + 1] units of the sequences before (per row), then the units of a work-group
+  float* part_o;    // [2 * work-groups][heads of a tile][D]
+  float* part_ml;   // [2 * work-groups][heads of a tile][2]
+  float* row_ml;    // [batch * heads][2], with weights
+  float* scores;    // [batch * heads][score_stride], NULL without weights
   float* weights;
   size_t w_sb, w_sh;
   size_t score_stride;
-  int heads, group, head_tiles, max_length, chunk, splits;
+  int batch, heads, group, head_tiles, tile_rows, max_length;
   float scaling;
 };
 
@@ -66,7 +78,9 @@ __device__ __forceinline__ float sum_over_groups(float v) {
 }
 
 // How a format's rows are read.  Keys: lane group g of a row takes kRun consecutive elements per load, kKeyLoads loads
-// 4 kRun apart.  Values: a lane takes c = D / 16 consecutive elements of each of its 8 slots.
+// 4 kRun apart.  Values: a lane takes c = D / 16 consecutive elements of each of its 8 slots.  kU pairs of 16-slot tiles
+// make a wavefront's step: as many as hold about the bytes of one pair of 16-bit rows of 128 (what a wavefront has in
+// flight covers the latency of HBM).
 template <int D, int FMT>
 struct Rows {
   static constexpr int kBits = FMT == MASE_KV_16BIT ? 16 : (FMT == MASE_KV_MXFP4 ? 4 : 8);
@@ -79,294 +93,467 @@ struct Rows {
   static constexpr int kValWords = kValBytes < 4 ? 1 : kValBytes / 4;
   static constexpr bool kPacked = FMT != MASE_KV_16BIT;
   static constexpr int kScaleWords = kPacked ? (D == 256 ? 2 : 1) : 1;
+  static constexpr int kU = (D * kBits >= 2048) ? 1 : (D * kBits >= 1024 ? MASE_PA_U8 : MASE_PA_U4);
+  static constexpr int kSlots = 32 * kU;             // per wavefront and step
+  static constexpr int kUnit = kWaves * kSlots;      // per work-group and step
+  static constexpr int kPerCu = D == 256 ? (kPacked ? 2 : 1) : (D == 64 ? MASE_PA_OCC + 1 : MASE_PA_OCC);    // work-groups that a CU holds (registers)
 };
 
-template <int D, int FMT, bool F16>
-__global__ __launch_bounds__(256) void paged_decode_kernel(DecodeParams p) {
+// units (work-group steps) of a sequence's row; a sequence without a slot has one too, which writes its zeros
+template <int UNIT>
+__device__ __forceinline__ int row_units(int length) {
+  return length > 0 ? (length + UNIT - 1) / UNIT : 1;
+}
+
+// The rows (sequence, cached head, head tile) with their units in one line are cut into equal shares, one for each
+// work-group of the launch, all of them resident: sequences of any lengths keep every CU busy to the end.  A row that lies
+// in one share is finished by it; the pieces of a row that is cut go to the share's first or last place (2 wg, 2 wg + 1)
+// and are joined by the second kernel.
+// EXTRA: with a mask or weights.
+template <int D, int FMT, bool F16, bool EXTRA>
+__global__ __launch_bounds__(256, (Rows<D, FMT>::kPerCu)) void paged_decode_kernel(DecodeParams p) {
   using R = Rows<D, FMT>;
+  constexpr int kU = R::kU;
   constexpr float kGrow = F16 ? 4.0f : 8.0f;   // see the reference point of the exponentials below
   constexpr float kShift = F16 ? 11.0f : 0.0f;
   extern __shared__ __attribute__((aligned(16))) float lds[];
+  __shared__ unsigned long long wave_sum[kWaves];
+  __shared__ int start_b, start_at;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int i = lane & 15, g = lane >> 4;
-  const int split = blockIdx.x, b = blockIdx.z;
-  const int hk = (int)blockIdx.y / p.head_tiles, tile = (int)blockIdx.y % p.head_tiles;
-  const int rows = min(kHeadTile, p.group - tile * kHeadTile);  // query heads here
-  const int head0 = hk * p.group + tile * kHeadTile;
-  const int length = kv_length(p.lengths[b], p.max_length, p.c.table_pages, p.c.page_shift);
-  const int lo = split * p.chunk, hi = min(lo + p.chunk, length);
-  if (split > 0 && lo >= length) return;  // an empty part; part 0 always reports
-  const int32_t* table = p.c.table + (size_t)b * p.c.table_stride;
   const int page_mask = (1 << p.c.page_shift) - 1;
+  const int row_heads = p.c.heads * p.head_tiles;  // rows of a sequence
+  auto length_of = [&](int b) __attribute__((always_inline)) { return kv_length(p.lengths[b], p.max_length, p.c.table_pages, p.c.page_shift); };
 
-  uint32_t qf[D / 32][4];
+  // this work-group's share [u0, u1) of all units, and where it starts
+  const int per = (p.batch + 255) / 256, b_lo = min((int)threadIdx.x * per, p.batch), b_hi = min(b_lo + per, p.batch);
+  unsigned long long mine = 0;
+  for (int b = b_lo; b < b_hi; ++b) mine += (unsigned)row_units<R::kUnit>(length_of(b));
+  unsigned long long run = mine;
 #pragma unroll
-  for (int u = 0; u < R::kKeyLoads; ++u)
+  for (int d = 1; d < 64; d <<= 1) {
+    const unsigned long long o = __shfl_up(run, d, 64);
+    if (lane >= d) run += o;
+  }
+  if (lane == 63) wave_sum[wave] = run;
+  __syncthreads();
+  unsigned long long before = run - mine, total = 0;
 #pragma unroll
-    for (int s = 0; s < R::kRun / 8; ++s) {
-      uint32_t* f = qf[u * (R::kRun / 8) + s];
-      if (i < rows) kv_load<16>(p.q + (size_t)b * p.q_sb + (size_t)(head0 + i) * p.q_sh + (u * 4 * R::kRun + g * R::kRun + s * 8) * 2, f);
-      else f[0] = f[1] = f[2] = f[3] = 0;
+  for (int w = 0; w < kWaves; ++w) {
+    before += w < wave ? wave_sum[w] : 0ull;
+    total += wave_sum[w];
+  }
+  const unsigned long long units = total * (unsigned)row_heads;
+  const unsigned long long share = (units + gridDim.x - 1) / gridDim.x;
+  const unsigned long long u0 = share * blockIdx.x, u1 = min(u0 + share, units);
+  if (blockIdx.x == 0) {
+    unsigned long long at = before;
+    for (int b = b_lo; b < b_hi; ++b) {
+      p.plan[b] = at;
+      at += (unsigned)row_units<R::kUnit>(length_of(b));
     }
-
-  // page and first row of the 16-slot tiles of a step (uniform); a page number that must not be followed reads page 0 and
-  // its slots count as absent
-  auto tile_page = [&](int slot, int& row) __attribute__((always_inline)) {
-    row = slot & page_mask;
-    return slot < hi ? kv_page(table, p.c.table_pages, p.c.page_shift, p.c.num_pages, slot) : -1;
-  };
-
-  uint32_t kr[2][R::kKeyLoads][R::kKeyWords], ksc[2][R::kScaleWords];
-  uint32_t vr[8][R::kValWords], vsc[2];
-  auto load_keys = [&](const int* page, const int* row) __attribute__((always_inline)) {
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int pg = max(page[t], 0);
-      const unsigned char* base = p.c.k + (size_t)pg * p.c.k_page + (size_t)hk * p.c.k_head + (size_t)row[t] * p.c.k_slot;
-#pragma unroll
-      for (int u = 0; u < R::kKeyLoads; ++u)
-        kv_load<R::kKeyBytes>(base + (uint32_t)i * p.c.k_slot + (uint32_t)((u * 4 + g) * R::kKeyBytes), kr[t][u]);
-      if constexpr (R::kPacked)
-        kv_load<D / 32>((const unsigned char*)p.c.ks + ((((size_t)pg * p.c.heads + hk) << p.c.page_shift) + row[t]) * (D / 32) + i * (D / 32), ksc[t]);
-    }
-  };
-  auto load_values = [&](const int* page, const int* row) __attribute__((always_inline)) {
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int pg = max(page[t], 0);
-      const unsigned char* base = p.c.v + (size_t)pg * p.c.v_page + (size_t)hk * p.c.v_head + (size_t)row[t] * p.c.v_slot;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        kv_load<R::kValBytes>(base + (uint32_t)(4 * g + j) * p.c.v_slot + (uint32_t)(i * R::kValBytes), vr[4 * t + j]);
-      if constexpr (R::kPacked)
-        vsc[t] = *(const uint32_t*)(p.c.vs + (((((size_t)pg * p.c.heads + hk) * (D / 32)) + (i * R::kC) / 32) << p.c.page_shift) + row[t] + 4 * g);
-    }
-  };
-
-  pa_f32x4_t o[R::kC];
-#pragma unroll
-  for (int n = 0; n < R::kC; ++n) o[n] = pa_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  float m = -__builtin_inff(), l = 0.0f;
-
-  for (int t0 = lo + wave * kSlots; t0 < hi; t0 += kChunkStep) {
-    int page[2], row[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) page[t] = tile_page(t0 + 16 * t, row[t]);
-    load_keys(page, row);
-    load_values(page, row);
-    // scores of head i at slots t0 + 16 t + 4 g + r
-    float x[2][4];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      pa_f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int u = 0; u < R::kKeyLoads; ++u) {
-        uint32_t wide[R::kRun / 2];
-        float scale = 0.0f;
-        if constexpr (R::kPacked) {
-          const int blk = (u * 4 * R::kRun + g * R::kRun) / 32;
-          const uint32_t word = R::kScaleWords == 1 ? ksc[t][0] : (blk < 4 ? ksc[t][0] : ksc[t][R::kScaleWords - 1]);
-          scale = kv_scale<FMT>((word >> (8 * (blk & 3))) & 0xFFu);
-        }
-        kv_widen<FMT, F16, R::kRun>(kr[t][u], scale, wide);
-#pragma unroll
-        for (int s = 0; s < R::kRun / 8; ++s) acc = mfma16<F16>(wide + 4 * s, qf[u * (R::kRun / 8) + s], acc);
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) x[t][r] = acc[r] * p.scaling;
-    }
-    const bool whole = t0 + kSlots <= hi && page[0] >= 0 && page[1] >= 0;
-    uint32_t gone = 0;  // bit 4 t + r: the slot is absent
-    if (!whole || p.mask != nullptr) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int slot = t0 + 16 * t + 4 * g + r;
-          bool absent = page[t] < 0 || slot >= hi;
-          if (p.mask != nullptr && !absent) {
-            const size_t at = (size_t)b * p.mask_sb + slot;
-            const float add = p.mask_f32 ? ((const float*)p.mask)[at] : DTypeTraits<F16 ? MASE_DT_F16 : MASE_DT_BF16>::load1(p.mask, at);
-            absent = add == -__builtin_inff();
-            x[t][r] += add;
-          }
-          if (absent) {
-            x[t][r] = -__builtin_inff();
-            gone |= 1u << (4 * t + r);
-          }
-        }
-    }
-    if (p.scores != nullptr && i < rows) {
-      float* sp = p.scores + ((size_t)b * p.heads + head0 + i) * p.score_stride + t0 + 4 * g;
-#pragma unroll
-      for (int t = 0; t < 2; ++t) *(float4*)(sp + 16 * t) = make_float4(x[t][0], x[t][1], x[t][2], x[t][3]);
-    }
-    // The reference point m of the exponentials moves only when some head has met a score more than kGrow (in the exponent's
-    // unit) above it: probabilities then reach 2^kGrow, and most steps skip the rescaling and the exchange between lanes.
-    float mx = x[0][0];
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) mx = fmaxf(mx, x[t][r]);
-    if (__builtin_amdgcn_ballot_w64((mx - m) * kLog2e > kGrow) != 0) {
-      const float mn = fmaxf(m, max_over_groups(mx));
-      const float alpha = mn == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * kLog2e);
-      m = mn;
-      l *= alpha;
-#pragma unroll
-      for (int n = 0; n < R::kC; ++n) o[n] *= alpha;
-    }
-    const float ms = m == -__builtin_inff() ? 0.0f : m;
-    // fp16 probabilities are held 2^kShift up, where small ones keep their bits (fp16 loses them below 2^-14)
-    uint32_t pf[4];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      float e[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        e[r] = __builtin_amdgcn_exp2f((x[t][r] - ms) * kLog2e + kShift);
-        l += e[r];
-      }
-      pf[2 * t] = kv_pack2<F16>(e[0], e[1]);
-      pf[2 * t + 1] = kv_pack2<F16>(e[2], e[3]);
-    }
-    // values: widened slot by slot, then pairs of slots joined
-    uint32_t wv[8][R::kC / 2];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float scale = R::kPacked ? kv_scale<FMT>((vsc[j >> 2] >> (8 * (j & 3))) & 0xFFu) : 0.0f;
-      kv_widen<FMT, F16, R::kC>(vr[j], scale, wv[j]);
-    }
-    if (gone != 0) {  // what an absent slot holds must not meet its probability of zero: it may be infinite or NaN
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if ((gone >> j) & 1u) {
-#pragma unroll
-          for (int n = 0; n < R::kC / 2; ++n) wv[j][n] = 0;
-        }
-    }
-#pragma unroll
-    for (int n = 0; n < R::kC; ++n) {
-      uint32_t f[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) f[q] = __builtin_amdgcn_perm(wv[2 * q + 1][n >> 1], wv[2 * q][n >> 1], (n & 1) ? 0x07060302u : 0x05040100u);
-      o[n] = mfma16<F16>(f, pf, o[n]);
+    if (threadIdx.x == 0) {
+      p.plan[p.batch] = total;
+      p.plan[p.batch + 1] = share;
     }
   }
-
-  // join the wavefronts: [wave][head] maxima and sums, [wave][head][D] outputs
-  l = sum_over_groups(l);
-  float* sm = lds;
-  float* sl = lds + kWaves * kHeadTile;
-  float* so = lds + 2 * kWaves * kHeadTile;
-  if (g == 0) {
-    sm[wave * kHeadTile + i] = m;
-    sl[wave * kHeadTile + i] = l;
-  }
-  if (i < rows) {
-    float* dst = so + (size_t)(wave * rows + i) * D;
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int n = 0; n < R::kC; n += 4)
-        *(float4*)(dst + R::kC * (4 * g + r) + n) = make_float4(o[n][r], o[n + 1][r], o[n + 2][r], o[n + 3][r]);
+  if (u0 >= u1) return;
+  if (before * (unsigned)row_heads <= u0 && u0 < (before + mine) * (unsigned)row_heads) {  // one thread
+    unsigned long long at = before * (unsigned)row_heads;
+    int b = b_lo;
+    for (; b < b_hi - 1; ++b) {
+      const unsigned long long n = (unsigned long long)(unsigned)row_units<R::kUnit>(length_of(b)) * (unsigned)row_heads;
+      if (u0 < at + n) break;
+      at += n;
+    }
+    start_b = b;
+    start_at = (int)(u0 - at);  // below units of a row * rows: see the host's limit
   }
   __syncthreads();
-  const bool direct = p.splits == 1 && p.scores == nullptr;
-  const float down = __builtin_amdgcn_exp2f(-kShift);
-  for (int e = threadIdx.x; e < rows * D; e += 256) {
-    const int r = e / D, d = e % D;
-    float top = sm[r];
+  int b = __builtin_amdgcn_readfirstlane(start_b);
+  int length = length_of(b), n_units = row_units<R::kUnit>(length);
+  int rh = min(__builtin_amdgcn_readfirstlane(start_at) / n_units, row_heads - 1), a = __builtin_amdgcn_readfirstlane(start_at) % n_units;
+  // units left, counted in 32 bits (the host's limit on the whole)
+  int left = __builtin_amdgcn_readfirstlane((int)(u1 - u0));
+
+#pragma unroll 1
+  for (bool first_piece = true;; first_piece = false) {
+    const int e = min(n_units, a + left);  // this row's units a .. e - 1
+    const int hk = rh / p.head_tiles, tile = rh % p.head_tiles;
+    const int rows = min(kHeadTile, p.group - tile * kHeadTile);  // query heads here
+    const int head0 = hk * p.group + tile * kHeadTile;
+    const int lo = a * R::kUnit, hi = min(e * R::kUnit, length);
+    const int32_t* table = p.c.table + (size_t)b * p.c.table_stride;
+
+    uint32_t qf[D / 32][4];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, sm[w * kHeadTile + r]);
-    float acc = 0.0f, sum = 0.0f;
+    for (int u = 0; u < R::kKeyLoads; ++u)
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float mw = sm[w * kHeadTile + r];
-      // a wavefront without a slot has m = -inf and zeros; one that met only NaN has them in its sums, which must show
-      const float f = mw == top ? 1.0f : __builtin_amdgcn_exp2f((mw - top) * kLog2e);
-      acc += f * so[(size_t)(w * rows + r) * D + d];
-      sum += f * sl[w * kHeadTile + r];
-    }
-    const size_t bh = (size_t)b * p.heads + head0 + r;
-    if (direct) {
-      const float y = sum == 0.0f ? 0.0f : acc / sum;
-      DTypeTraits<F16 ? MASE_DT_F16 : MASE_DT_BF16>::store1(p.out, bh * D + d, y);
-    } else {
-      p.part_o[(bh * p.splits + split) * D + d] = acc * down;
-      if (d == 0) {
-        p.part_ml[(bh * p.splits + split) * 2] = top;
-        p.part_ml[(bh * p.splits + split) * 2 + 1] = sum * down;
+      for (int s = 0; s < R::kRun / 8; ++s) {
+        uint32_t* f = qf[u * (R::kRun / 8) + s];
+        if (i < rows) kv_load<16>(p.q + (size_t)b * p.q_sb + (size_t)(head0 + i) * p.q_sh + (u * 4 * R::kRun + g * R::kRun + s * 8) * 2, f);
+        else f[0] = f[1] = f[2] = f[3] = 0;
       }
+
+    // page and first row of a 16-slot tile (uniform); a page number that must not be followed reads page 0 and its slots
+    // count as absent
+    auto tile_page = [&](int slot, int& row) __attribute__((always_inline)) {
+      row = slot & page_mask;
+      return slot < hi ? kv_page(table, p.c.table_pages, p.c.page_shift, p.c.num_pages, slot) : -1;
+    };
+    uint32_t kr[2 * kU][R::kKeyLoads][R::kKeyWords], ksc[2 * kU][R::kScaleWords];
+    uint32_t vr[8 * kU][R::kValWords], vsc[2 * kU];
+    float mk[2 * kU][4];
+    auto load_keys = [&](const int* page, const int* row) __attribute__((always_inline)) {
+#pragma unroll
+      for (int t = 0; t < 2 * kU; ++t) {
+        const int pg = max(page[t], 0);
+        const unsigned char* base = p.c.k + (size_t)pg * p.c.k_page + (size_t)hk * p.c.k_head + (size_t)row[t] * p.c.k_slot;
+#pragma unroll
+        for (int u = 0; u < R::kKeyLoads; ++u)
+          kv_load<R::kKeyBytes>(base + (uint32_t)i * p.c.k_slot + (uint32_t)((u * 4 + g) * R::kKeyBytes), kr[t][u]);
+        if constexpr (R::kPacked)
+          kv_load<D / 32>((const unsigned char*)p.c.ks + ((((size_t)pg * p.c.heads + hk) << p.c.page_shift) + row[t]) * (D / 32) + i * (D / 32), ksc[t]);
+      }
+    };
+    auto load_values = [&](const int* page, const int* row) __attribute__((always_inline)) {
+#pragma unroll
+      for (int t = 0; t < 2 * kU; ++t) {
+        const int pg = max(page[t], 0);
+        const unsigned char* base = p.c.v + (size_t)pg * p.c.v_page + (size_t)hk * p.c.v_head + (size_t)row[t] * p.c.v_slot;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          kv_load<R::kValBytes>(base + (uint32_t)(4 * g + j) * p.c.v_slot + (uint32_t)(i * R::kValBytes), vr[4 * t + j]);
+        if constexpr (R::kPacked)
+          vsc[t] = *(const uint32_t*)(p.c.vs + (((((size_t)pg * p.c.heads + hk) * (D / 32)) + (i * R::kC) / 32) << p.c.page_shift) + row[t] + 4 * g);
+      }
+    };
+    // what is added to the scores of slots s0 + 16 t + 4 g + r (slots past the end read the last one's)
+    auto load_mask = [&](int s0) __attribute__((always_inline)) {
+      if constexpr (EXTRA) {
+        if (p.mask == nullptr) return;
+#pragma unroll
+        for (int t = 0; t < 2 * kU; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const size_t at = (size_t)b * p.mask_sb + (size_t)min(s0 + 16 * t + 4 * g + r, hi - 1);
+            mk[t][r] = p.mask_f32 ? ((const float*)p.mask)[at] : DTypeTraits<F16 ? MASE_DT_F16 : MASE_DT_BF16>::load1(p.mask, at);
+          }
+      }
+    };
+
+    pa_f32x4_t o[R::kC];
+#pragma unroll
+    for (int n = 0; n < R::kC; ++n) o[n] = pa_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -__builtin_inff(), l = 0.0f;
+
+    // A step's keys are read while the step before turns scores into outputs, its values while the step itself computes the
+    // scores: each overwrites the registers that were just used, so the loads need none of their own.  Page numbers are read
+    // one step further ahead.  Past the end the last step's rows are read again (from the cache), which keeps the count of
+    // loads in flight the same on every path.
+    int page[2 * kU], row[2 * kU], page_n[2 * kU], row_n[2 * kU];
+    const int first = lo + wave * R::kSlots;
+    if (first < hi) {
+#pragma unroll
+      for (int t = 0; t < 2 * kU; ++t) {
+        page[t] = tile_page(first + 16 * t, row[t]);
+        page_n[t] = tile_page(first + R::kUnit + 16 * t, row_n[t]);
+      }
+      load_mask(first);
+      load_keys(page, row);
+      load_values(page, row);
+    }
+    for (int t0 = first; t0 < hi; t0 += R::kUnit) {
+      const bool more = t0 + R::kUnit < hi;
+      // scores of head i at slots t0 + 16 t + 4 g + r
+      float x[2 * kU][4];
+#pragma unroll
+      for (int t = 0; t < 2 * kU; ++t) {
+        pa_f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int u = 0; u < R::kKeyLoads; ++u) {
+          uint32_t wide[R::kRun / 2];
+          float scale = 0.0f;
+          if constexpr (R::kPacked) {
+            const int blk = (u * 4 * R::kRun + g * R::kRun) / 32;
+            const uint32_t word = R::kScaleWords == 1 ? ksc[t][0] : (blk < 4 ? ksc[t][0] : ksc[t][R::kScaleWords - 1]);
+            scale = kv_scale<FMT>((word >> (8 * (blk & 3))) & 0xFFu);
+          }
+          kv_widen<FMT, F16, R::kRun>(kr[t][u], scale, wide);
+#pragma unroll
+          for (int s = 0; s < R::kRun / 8; ++s) acc = mfma16<F16>(wide + 4 * s, qf[u * (R::kRun / 8) + s], acc);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[t][r] = acc[r] * p.scaling;
+        if (kU > 1) __builtin_amdgcn_sched_barrier(0);
+      }
+      bool whole = t0 + R::kSlots <= hi;
+#pragma unroll
+      for (int t = 0; t < 2 * kU; ++t) whole = whole && page[t] >= 0;
+      uint32_t gone = 0;  // bit 4 t + r: the slot is absent
+      if (EXTRA && p.mask != nullptr) {
+#pragma unroll
+        for (int t = 0; t < 2 * kU; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            x[t][r] += mk[t][r];
+            if (mk[t][r] == -__builtin_inff()) gone |= 1u << (4 * t + r);
+          }
+      }
+      if (!whole) {
+#pragma unroll
+        for (int t = 0; t < 2 * kU; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (page[t] < 0 || t0 + 16 * t + 4 * g + r >= hi) gone |= 1u << (4 * t + r);
+      }
+      if (EXTRA || !whole) {
+#pragma unroll
+        for (int t = 0; t < 2 * kU; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if ((gone >> (4 * t + r)) & 1u) x[t][r] = -__builtin_inff();
+      }
+#pragma unroll
+      for (int t = 0; t < 2 * kU; ++t) {  // the next step's pages, or the same again
+        page[t] = more ? page_n[t] : page[t];
+        row[t] = more ? row_n[t] : row[t];
+      }
+      load_mask(more ? t0 + R::kUnit : t0);
+      load_keys(page, row);
+#pragma unroll
+      for (int t = 0; t < 2 * kU; ++t) page_n[t] = tile_page(t0 + 2 * R::kUnit + 16 * t, row_n[t]);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (EXTRA) {
+        if (p.scores != nullptr && i < rows) {
+          float* sp = p.scores + ((size_t)b * p.heads + head0 + i) * p.score_stride + t0 + 4 * g;
+#pragma unroll
+          for (int t = 0; t < 2 * kU; ++t) *(float4*)(sp + 16 * t) = make_float4(x[t][0], x[t][1], x[t][2], x[t][3]);
+        }
+      }
+      // The reference point m of the exponentials moves only when some head has met a score more than kGrow (in the
+      // exponent's unit) above it: probabilities then reach 2^kGrow, and most steps skip the rescaling and the exchange
+      // between lanes.
+      float mx = x[0][0];
+#pragma unroll
+      for (int t = 0; t < 2 * kU; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, x[t][r]);
+      if (__builtin_amdgcn_ballot_w64((mx - m) * kLog2e > kGrow) != 0) {
+        const float mn = fmaxf(m, max_over_groups(mx));
+        const float alpha = mn == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * kLog2e);
+        m = mn;
+        l *= alpha;
+#pragma unroll
+        for (int n = 0; n < R::kC; ++n) o[n] *= alpha;
+      }
+      const float ms = m == -__builtin_inff() ? 0.0f : m;
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        // fp16 probabilities are held 2^kShift up, where small ones keep their bits (fp16 loses them below 2^-14)
+        uint32_t pf[4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          float ex[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            ex[r] = __builtin_amdgcn_exp2f((x[2 * u + t][r] - ms) * kLog2e + kShift);
+            l += ex[r];
+          }
+          pf[2 * t] = kv_pack2<F16>(ex[0], ex[1]);
+          pf[2 * t + 1] = kv_pack2<F16>(ex[2], ex[3]);
+        }
+        // values: widened slot by slot, then pairs of slots joined
+        uint32_t wv[8][R::kC / 2];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float scale = R::kPacked ? kv_scale<FMT>((vsc[2 * u + (j >> 2)] >> (8 * (j & 3))) & 0xFFu) : 0.0f;
+          kv_widen<FMT, F16, R::kC>(vr[8 * u + j], scale, wv[j]);
+        }
+        if (EXTRA || !whole) {  // what an absent slot holds must not meet its probability of zero: it may be infinite or NaN
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if ((gone >> (8 * u + j)) & 1u) {
+#pragma unroll
+              for (int n = 0; n < R::kC / 2; ++n) wv[j][n] = 0;
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < R::kC; ++n) {
+          uint32_t f[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) f[q] = __builtin_amdgcn_perm(wv[2 * q + 1][n >> 1], wv[2 * q][n >> 1], (n & 1) ? 0x07060302u : 0x05040100u);
+          o[n] = mfma16<F16>(f, pf, o[n]);
+        }
+        if (kU > 1) __builtin_amdgcn_sched_barrier(0);
+      }
+      load_values(page, row);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+
+    // join the wavefronts: [wave][head] maxima and sums, [wave][head][D] outputs
+    l = sum_over_groups(l);
+    float* sm = lds;
+    float* sl = lds + kWaves * kHeadTile;
+    float* so = lds + 2 * kWaves * kHeadTile;
+    if (g == 0) {
+      sm[wave * kHeadTile + i] = m;
+      sl[wave * kHeadTile + i] = l;
+    }
+    if (i < rows) {
+      float* dst = so + (size_t)(wave * rows + i) * D;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int n = 0; n < R::kC; n += 4)
+          *(float4*)(dst + R::kC * (4 * g + r) + n) = make_float4(o[n][r], o[n + 1][r], o[n + 2][r], o[n + 3][r]);
+    }
+    __syncthreads();
+    const bool all = a == 0 && e == n_units;
+    const float down = __builtin_amdgcn_exp2f(-kShift);
+    const size_t place = 2 * (size_t)blockIdx.x + (first_piece ? 0 : 1);
+    for (int el = threadIdx.x; el < rows * D; el += 256) {
+      const int r = el / D, d = el % D;
+      float top = sm[r];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) top = fmaxf(top, sm[w * kHeadTile + r]);
+      float acc = 0.0f, sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float mw = sm[w * kHeadTile + r];
+        // a wavefront without a slot has m = -inf and zeros; one that met only NaN has them in its sums, which must show
+        const float f = mw == top ? 1.0f : __builtin_amdgcn_exp2f((mw - top) * kLog2e);
+        acc += f * so[(size_t)(w * rows + r) * D + d];
+        sum += f * sl[w * kHeadTile + r];
+      }
+      const size_t bh = (size_t)b * p.heads + head0 + r;
+      float* ml = nullptr;
+      if (all) {
+        const float y = sum == 0.0f ? 0.0f : acc / sum;
+        DTypeTraits<F16 ? MASE_DT_F16 : MASE_DT_BF16>::store1(p.out, bh * D + d, y);
+        if (EXTRA && p.scores != nullptr) ml = p.row_ml + bh * 2;
+      } else {
+        p.part_o[(place * p.tile_rows + r) * D + d] = acc * down;
+        ml = p.part_ml + (place * p.tile_rows + r) * 2;
+      }
+      if (ml != nullptr && d == 0) {
+        ml[0] = top;
+        ml[1] = sum * down;
+      }
+    }
+    left -= e - a;
+    if (left <= 0) break;
+    __syncthreads();  // everyone has read the LDS
+    a = 0;
+    if (++rh == row_heads) {
+      rh = 0;
+      if (++b >= p.batch) break;  // lengths that change under the kernel must not lead past the last sequence
+      length = length_of(b);
+      n_units = row_units<R::kUnit>(length);
     }
   }
 }
 
-// Joins the parts.  grid (x, cached head, sequence): a work-group takes the query heads x, x + gridDim.x, ... of its cached
-// head and, with weights, the slots of its share.
+// The pieces of row `rh` of sequence b: how many (1: the row was finished in one piece), and where piece k lies.
+struct Pieces {
+  int count;
+  unsigned long long wg0;
+  bool from_start;
+  __device__ __forceinline__ size_t place(int k) const { return 2 * (size_t)(wg0 + k) + (k == 0 && !from_start ? 1 : 0); }
+};
+__device__ __forceinline__ Pieces row_pieces(const DecodeParams& p, int b, int rh, int row_heads) {
+  const unsigned long long before = p.plan[b], n = p.plan[b + 1] - before, share = p.plan[p.batch + 1];
+  const unsigned long long at = before * (unsigned)row_heads + (unsigned long long)rh * n;
+  Pieces q;
+  q.wg0 = at / share;
+  q.from_start = q.wg0 * share == at;
+  q.count = (int)((at + n - 1) / share - q.wg0) + 1;
+  return q;
+}
+
+// max and sum over the pieces of one head, by one wavefront
+__device__ __forceinline__ void head_ml(const DecodeParams& p, const Pieces& q, int r, int lane, float& top, float& sum) {
+  top = -__builtin_inff();
+  for (int k = lane; k < q.count; k += 64) top = fmaxf(top, p.part_ml[(q.place(k) * p.tile_rows + r) * 2]);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+  sum = 0.0f;
+  for (int k = lane; k < q.count; k += 64) {
+    const float* ml = p.part_ml + (q.place(k) * p.tile_rows + r) * 2;
+    sum += ml[1] * (ml[0] == top ? 1.0f : __builtin_amdgcn_exp2f((ml[0] - top) * kLog2e));
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
+}
+
 constexpr int kMaxGroup = 256;
 constexpr int kWeightSlots = 1024;  // per work-group
+constexpr int kJoinCols = 32;       // of the head dimension per work-group
 
+// Joins the pieces of cut rows (blocks x < joins: one query head of the cached head and kJoinCols columns each) and, with
+// weights, adds the probabilities of kWeightSlots slots (the blocks behind).  grid (x, cached head, sequence).
 template <int D, bool F16>
-__global__ __launch_bounds__(256) void paged_decode_join_kernel(DecodeParams p) {
+__global__ __launch_bounds__(256) void paged_decode_join_kernel(DecodeParams p, int joins) {
   __shared__ float top_s[kMaxGroup], inv_s[kMaxGroup];
   __shared__ __attribute__((aligned(16))) float red[256 * 4];
   const int hk = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int length = kv_length(p.lengths[b], p.max_length, p.c.table_pages, p.c.page_shift);
-  const int parts = max(1, (length + p.chunk - 1) / p.chunk);
+  const int row_heads = p.c.heads * p.head_tiles;
   const size_t bh0 = (size_t)b * p.heads + (size_t)hk * p.group;
-  const int step = (int)gridDim.x;
-  const bool all = p.scores != nullptr;
-  // reference point and 1 / sum of each head that this work-group needs
+  if ((int)blockIdx.x < joins) {
+    const int h = (int)blockIdx.x / (D / kJoinCols), col0 = ((int)blockIdx.x % (D / kJoinCols)) * kJoinCols;
+    const Pieces q = row_pieces(p, b, hk * p.head_tiles + h / kHeadTile, row_heads);
+    if (q.count == 1) return;
+    const int r = h % kHeadTile;
+    float top, sum;
+    head_ml(p, q, r, lane, top, sum);  // every wavefront for itself
+    constexpr int kCols = kJoinCols / 4, kRows = 256 / kCols;  // threads along the columns, pieces side by side
+    const int col = tid % kCols, at = tid / kCols;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int k = at; k < q.count; k += kRows) {
+      const size_t place = q.place(k) * p.tile_rows + r;
+      const float mk = p.part_ml[place * 2];
+      const float4 v = *(const float4*)(p.part_o + place * D + col0 + col * 4);
+      const float f = mk == top ? 1.0f : __builtin_amdgcn_exp2f((mk - top) * kLog2e);
+      acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
+    }
+    ((float4*)red)[tid] = acc;
+    __syncthreads();
+    if (tid < kCols) {
+      for (int k = 1; k < kRows; ++k) {
+        const float4 v = ((const float4*)red)[k * kCols + tid];
+        acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+      }
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      uint2 y;
+      y.x = kv_pack2<F16>(acc.x * inv, acc.y * inv);
+      y.y = kv_pack2<F16>(acc.z * inv, acc.w * inv);
+      *(uint2*)(p.out + ((bh0 + h) * D + col0 + tid * 4) * 2) = y;
+    }
+    return;
+  }
+  const int s0 = ((int)blockIdx.x - joins) * kWeightSlots;
+  const int length = kv_length(p.lengths[b], p.max_length, p.c.table_pages, p.c.page_shift);
+  if (s0 >= length) return;
   for (int h = wave; h < p.group; h += 4) {
-    if (!all && h % step != (int)blockIdx.x) continue;
-    const float* ml = p.part_ml + (bh0 + h) * p.splits * 2;
-    float top = -__builtin_inff();
-    for (int s = lane; s < parts; s += 64) top = fmaxf(top, ml[2 * s]);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-    float sum = 0.0f;
-    for (int s = lane; s < parts; s += 64) sum += ml[2 * s + 1] * (ml[2 * s] == top ? 1.0f : __builtin_amdgcn_exp2f((ml[2 * s] - top) * kLog2e));
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
+    const Pieces q = row_pieces(p, b, hk * p.head_tiles + h / kHeadTile, row_heads);
+    float top, sum;
+    if (q.count == 1) {
+      top = p.row_ml[(bh0 + h) * 2];
+      sum = p.row_ml[(bh0 + h) * 2 + 1];
+    } else {
+      head_ml(p, q, h % kHeadTile, lane, top, sum);
+    }
     if (lane == 0) {
       top_s[h] = top;
       inv_s[h] = sum == 0.0f ? 0.0f : 1.0f / sum;
     }
   }
   __syncthreads();
-  constexpr int kCols = D / 4, kRows = 256 / kCols;  // threads along the head dimension, parts side by side
-  const int col = tid % kCols, rowi = tid / kCols;
-  for (int h = blockIdx.x; h < p.group; h += step) {
-    const float* ml = p.part_ml + (bh0 + h) * p.splits * 2;
-    const float* po = p.part_o + (bh0 + h) * p.splits * D + col * 4;
-    const float top = top_s[h];
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int s = rowi; s < parts; s += kRows) {
-      const float f = ml[2 * s] == top ? 1.0f : __builtin_amdgcn_exp2f((ml[2 * s] - top) * kLog2e);
-      const float4 v = *(const float4*)(po + (size_t)s * D);
-      acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
-    }
-    ((float4*)red)[tid] = acc;
-    __syncthreads();
-    if (tid < kCols) {
-      for (int r = 1; r < kRows; ++r) {
-        const float4 v = ((const float4*)red)[r * kCols + tid];
-        acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
-      }
-      const float inv = inv_s[h];
-      uint2 y;
-      y.x = kv_pack2<F16>(acc.x * inv, acc.y * inv);
-      y.y = kv_pack2<F16>(acc.z * inv, acc.w * inv);
-      *(uint2*)(p.out + ((bh0 + h) * D + tid * 4) * 2) = y;
-    }
-    __syncthreads();
-  }
-  if (!all) return;
   float* wrow = p.weights + (size_t)b * p.w_sb + (size_t)hk * p.w_sh;
-  const int end = min(length, ((int)blockIdx.x + 1) * kWeightSlots);
-  for (int s = (int)blockIdx.x * kWeightSlots + tid; s < end; s += 256) {
+  const int end = min(length, s0 + kWeightSlots);
+  for (int s = s0 + tid; s < end; s += 256) {
     float acc = 0.0f;
     for (int h = 0; h < p.group; ++h) {
       const float x = p.scores[(bh0 + h) * p.score_stride + s];
@@ -377,79 +564,122 @@ __global__ __launch_bounds__(256) void paged_decode_join_kernel(DecodeParams p) 
   }
 }
 
+// What a call launches and keeps between its two kernels.
 struct DecodePlan {
-  int chunk, splits, head_tiles;
-  size_t score_stride, part_floats, ml_floats, score_floats;
+  int groups;      // work-groups
+  int head_tiles, tile_rows;
+  bool join;       // a row may be cut
+  size_t score_stride, plan_bytes, part_floats, ml_floats, row_ml_floats, score_floats;
+  size_t bytes() const { return plan_bytes + (part_floats + ml_floats + row_ml_floats + score_floats) * sizeof(float); }
 };
 
-// How the cache's length is split: parts of a whole number of work-group steps, about kPartsPerCu work-groups per CU when
-// all sequences are as long as the longest may be.
-constexpr int kPartsPerCu = 8;
-
-DecodePlan decode_plan(size_t batch, size_t heads, size_t kv_heads, size_t head_dim, size_t max_length, bool weights) {
+template <int D, int FMT>
+DecodePlan decode_plan(size_t batch, size_t heads, size_t kv_heads, size_t max_length, bool weights) {
+  using R = Rows<D, FMT>;
   DecodePlan d{};
   const size_t group = heads / kv_heads;
   d.head_tiles = (int)((group + kHeadTile - 1) / kHeadTile);
+  d.tile_rows = (int)(group < kHeadTile ? group : kHeadTile);
   int cus = device_cu_count();
   if (cus <= 0) cus = 256;
-  const size_t rows = batch * kv_heads * d.head_tiles;
-  const size_t steps = (max_length + kChunkStep - 1) / kChunkStep;
-  size_t splits = (size_t)cus * kPartsPerCu / (rows ? rows : 1);
-  if (splits < 1) splits = 1;
-  if (splits > steps) splits = steps ? steps : 1;
-  const size_t per = steps ? (steps + splits - 1) / splits : 1;
-  d.chunk = (int)(per * kChunkStep);
-  d.splits = (int)(steps ? (steps + per - 1) / per : 1);
-  d.score_stride = steps * kChunkStep;
-  const bool join = d.splits > 1 || weights;
-  d.part_floats = join ? batch * heads * d.splits * head_dim : 0;
-  d.ml_floats = join ? (batch * heads * d.splits * 2 + 3) / 4 * 4 : 0;
+  const size_t steps = max_length ? (max_length + R::kUnit - 1) / R::kUnit : 1;
+  const size_t most = batch * kv_heads * d.head_tiles * steps;
+  d.groups = (int)(most < (size_t)cus * R::kPerCu * MASE_PA_ROUNDS ? most : (size_t)cus * R::kPerCu * MASE_PA_ROUNDS);
+  d.join = steps > 1;
+  d.score_stride = steps * R::kUnit;
+  d.plan_bytes = (batch + 2 + 1) / 2 * 2 * sizeof(unsigned long long);
+  d.part_floats = d.join ? 2 * (size_t)d.groups * d.tile_rows * D : 0;
+  d.ml_floats = d.join ? 2 * (size_t)d.groups * d.tile_rows * 2 : 0;
+  d.row_ml_floats = weights ? (batch * heads * 2 + 3) / 4 * 4 : 0;
   d.score_floats = weights ? batch * heads * d.score_stride : 0;
   return d;
 }
 
-template <int D, int FMT, bool F16>
-int launch_decode(const DecodeParams& p, size_t batch, hipStream_t st) {
-  const int lds = (int)sizeof(float) * (2 * kWaves * kHeadTile + kWaves * min(p.group, kHeadTile) * D);
+template <int D, int FMT, bool F16, bool EXTRA>
+int launch_decode(const DecodeParams& p, const DecodePlan& d, hipStream_t st) {
+  const size_t lds = sizeof(float) * (2 * kWaves * kHeadTile + (size_t)kWaves * d.tile_rows * D);
   static std::atomic<uint64_t> attr_done{0};
-  const void* fn = (const void*)paged_decode_kernel<D, FMT, F16>;
+  const void* fn = (const void*)paged_decode_kernel<D, FMT, F16, EXTRA>;
   if (!set_dynamic_lds_once(attr_done, fn, (int)sizeof(float) * (2 * kWaves * kHeadTile + kWaves * kHeadTile * D))) return MASE_ERR_LAUNCH;
-  const dim3 grid((unsigned)p.splits, (unsigned)(p.c.heads * p.head_tiles), (unsigned)batch);
-  hipLaunchKernelGGL((paged_decode_kernel<D, FMT, F16>), grid, dim3(256), (size_t)lds, st, p);
+  hipLaunchKernelGGL((paged_decode_kernel<D, FMT, F16, EXTRA>), dim3((unsigned)d.groups), dim3(256), lds, st, p);
+  const bool weights = p.scores != nullptr;
+  if (!d.join && !weights) return MASE_OK;
+  const unsigned joins = d.join ? (unsigned)(p.group * (D / kJoinCols)) : 0;
+  const unsigned shares = weights ? blocks_for((size_t)p.max_length, kWeightSlots) : 0;
+  if (joins + shares > 0)
+    hipLaunchKernelGGL((paged_decode_join_kernel<D, F16>), dim3(joins + shares, (unsigned)p.c.heads, (unsigned)p.batch), dim3(256), 0, st, p, (int)joins);
   return MASE_OK;
 }
 
-template <int D>
-int launch_decode_d(const DecodeParams& p, int format, bool f16, size_t batch, hipStream_t st) {
-  int rc;
-  switch (format * 2 + (f16 ? 1 : 0)) {
-    case MASE_KV_16BIT * 2: rc = launch_decode<D, MASE_KV_16BIT, false>(p, batch, st); break;
-    case MASE_KV_16BIT * 2 + 1: rc = launch_decode<D, MASE_KV_16BIT, true>(p, batch, st); break;
-    case MASE_KV_MXINT8 * 2: rc = launch_decode<D, MASE_KV_MXINT8, false>(p, batch, st); break;
-    case MASE_KV_MXINT8 * 2 + 1: rc = launch_decode<D, MASE_KV_MXINT8, true>(p, batch, st); break;
-    case MASE_KV_MXFP8_E4M3 * 2: rc = launch_decode<D, MASE_KV_MXFP8_E4M3, false>(p, batch, st); break;
-    case MASE_KV_MXFP8_E4M3 * 2 + 1: rc = launch_decode<D, MASE_KV_MXFP8_E4M3, true>(p, batch, st); break;
-    case MASE_KV_MXFP8_E5M2 * 2: rc = launch_decode<D, MASE_KV_MXFP8_E5M2, false>(p, batch, st); break;
-    case MASE_KV_MXFP8_E5M2 * 2 + 1: rc = launch_decode<D, MASE_KV_MXFP8_E5M2, true>(p, batch, st); break;
-    case MASE_KV_MXFP4 * 2: rc = launch_decode<D, MASE_KV_MXFP4, false>(p, batch, st); break;
-    default: rc = launch_decode<D, MASE_KV_MXFP4, true>(p, batch, st); break;
+struct DecodeCall {  // a call's arguments; workspace_bytes == NULL: launch, else only say how much workspace it takes
+  DecodeParams p;
+  size_t batch, heads, kv_heads, max_length;
+  bool f16, extra, with_weights;
+  unsigned char* workspace;
+  size_t workspace_bytes;
+  size_t* need;
+  hipStream_t st;
+};
+
+template <int D, int FMT>
+int decode_call(DecodeCall& c) {
+  const DecodePlan d = decode_plan<D, FMT>(c.batch, c.heads, c.kv_heads, c.max_length, c.with_weights);
+  if (c.need != nullptr) {
+    *c.need = d.bytes();
+    return MASE_OK;
   }
-  if (rc != MASE_OK || p.part_o == nullptr) return rc;
-  const size_t shares = p.scores != nullptr ? ((size_t)p.max_length + kWeightSlots - 1) / kWeightSlots : (size_t)p.group;
-  const dim3 grid((unsigned)(shares ? shares : 1), (unsigned)p.c.heads, (unsigned)batch);
-  if (f16) hipLaunchKernelGGL((paged_decode_join_kernel<D, true>), grid, dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((paged_decode_join_kernel<D, false>), grid, dim3(256), 0, st, p);
-  return MASE_OK;
+  if (c.workspace == nullptr || c.workspace_bytes < d.bytes()) return MASE_ERR_WORKSPACE;
+  if (!aligned16(c.workspace)) return MASE_ERR_ALIGN;
+  // a place within one sequence's rows, and a work-group's share with a row's units on top, are counted in 32 bits
+  const size_t row = c.max_length / Rows<D, FMT>::kUnit + 1, rows = c.kv_heads * d.head_tiles;
+  if (row * rows > 0x3FFFFFFFu || c.batch * rows * row / (size_t)d.groups > 0x3FFFFFFEu) return MASE_ERR_SHAPE;
+  c.p.plan = (unsigned long long*)c.workspace;
+  float* f = (float*)(c.workspace + d.plan_bytes);
+  c.p.part_o = f;
+  c.p.part_ml = f + d.part_floats;
+  c.p.row_ml = c.p.part_ml + d.ml_floats;
+  c.p.scores = c.with_weights ? c.p.row_ml + d.row_ml_floats : nullptr;
+  c.p.score_stride = d.score_stride;
+  c.p.head_tiles = d.head_tiles;
+  c.p.tile_rows = d.tile_rows;
+  if (c.f16) return c.extra ? launch_decode<D, FMT, true, true>(c.p, d, c.st) : launch_decode<D, FMT, true, false>(c.p, d, c.st);
+  return c.extra ? launch_decode<D, FMT, false, true>(c.p, d, c.st) : launch_decode<D, FMT, false, false>(c.p, d, c.st);
+}
+
+int decode_dispatch(size_t head_dim, int format, DecodeCall& c) {
+  switch ((int)head_dim * 8 + format) {
+#define MASE_PA_CASES(D)                                                            \
+  case D * 8 + MASE_KV_16BIT: return decode_call<D, MASE_KV_16BIT>(c);              \
+  case D * 8 + MASE_KV_MXINT8: return decode_call<D, MASE_KV_MXINT8>(c);            \
+  case D * 8 + MASE_KV_MXFP8_E4M3: return decode_call<D, MASE_KV_MXFP8_E4M3>(c);    \
+  case D * 8 + MASE_KV_MXFP8_E5M2: return decode_call<D, MASE_KV_MXFP8_E5M2>(c);    \
+  case D * 8 + MASE_KV_MXFP4: return decode_call<D, MASE_KV_MXFP4>(c);
+    MASE_PA_CASES(64)
+    MASE_PA_CASES(128)
+    MASE_PA_CASES(256)
+#undef MASE_PA_CASES
+    default: return MASE_ERR_SHAPE;
+  }
 }
 
 }  // namespace
 }  // namespace mase
 
 extern "C" size_t mase_paged_attention_decode_workspace_bytes(size_t batch, size_t heads, size_t kv_heads, size_t head_dim,
-                                                              size_t max_length, int with_weights) {
-  if (kv_heads == 0 || heads % kv_heads != 0 || max_length > 0x7FFFFF00u) return 0;
-  const mase::DecodePlan d = mase::decode_plan(batch, heads, kv_heads, head_dim, max_length, with_weights != 0);
-  return (d.part_floats + d.ml_floats + d.score_floats) * sizeof(float);
+                                                              int format, size_t max_length, int with_weights) {
+  using namespace mase;
+  if (batch == 0 || batch > 65535 || kv_heads == 0 || heads == 0 || heads % kv_heads != 0 || heads / kv_heads > (size_t)kMaxGroup ||
+      max_length > 0x7FFFFF00u || (head_dim != 64 && head_dim != 128 && head_dim != 256))
+    return 0;
+  size_t need = 0;
+  DecodeCall c{};
+  c.batch = batch;
+  c.heads = heads;
+  c.kv_heads = kv_heads;
+  c.max_length = max_length;
+  c.with_weights = with_weights != 0;
+  c.need = &need;
+  return decode_dispatch(head_dim, format, c) == MASE_OK ? need : 0;
 }
 
 extern "C" int mase_paged_attention_decode(const mase_paged_kv* cache, const void* q, size_t q_stride_b, size_t q_stride_h,
@@ -458,7 +688,8 @@ extern "C" int mase_paged_attention_decode(const mase_paged_kv* cache, const voi
                                            size_t w_stride_b, size_t w_stride_h, void* out, void* workspace,
                                            size_t workspace_bytes, void* stream) {
   using namespace mase;
-  DecodeParams p{};
+  DecodeCall call{};
+  DecodeParams& p = call.p;
   const int rc = paged_kv_params(cache, p.c);
   if (rc != MASE_OK) return rc;
   if (heads == 0 || heads % cache->kv_heads != 0 || heads / cache->kv_heads > (size_t)kMaxGroup) return MASE_ERR_SHAPE;
@@ -468,11 +699,6 @@ extern "C" int mase_paged_attention_decode(const mase_paged_kv* cache, const voi
   if (cache->batch == 0) return MASE_OK;
   if (q == nullptr || lengths == nullptr || out == nullptr) return MASE_ERR_NULL;
   if (!aligned16(q) || !aligned16(out) || q_stride_b % 8 != 0 || q_stride_h % 8 != 0) return MASE_ERR_ALIGN;
-  const DecodePlan d = decode_plan(cache->batch, heads, cache->kv_heads, cache->head_dim, max_length, weights != nullptr);
-  if (cache->kv_heads * d.head_tiles > 65535) return MASE_ERR_SHAPE;
-  const size_t need = (d.part_floats + d.ml_floats + d.score_floats) * sizeof(float);
-  if (need != 0 && (workspace == nullptr || workspace_bytes < need)) return MASE_ERR_WORKSPACE;
-  if (need != 0 && !aligned16(workspace)) return MASE_ERR_ALIGN;
   p.q = (const unsigned char*)q;
   p.q_sb = q_stride_b * 2;
   p.q_sh = q_stride_h * 2;
@@ -481,28 +707,25 @@ extern "C" int mase_paged_attention_decode(const mase_paged_kv* cache, const voi
   p.mask_sb = mask_stride_b;
   p.mask_f32 = mask_dtype == MASE_DT_F32;
   p.out = (unsigned char*)out;
-  if (need != 0) {
-    p.part_o = (float*)workspace;
-    p.part_ml = p.part_o + d.part_floats;
-    p.scores = weights != nullptr ? p.part_ml + d.ml_floats : nullptr;
-  }
   p.weights = weights;
   p.w_sb = w_stride_b;
   p.w_sh = w_stride_h;
-  p.score_stride = d.score_stride;
+  p.batch = (int)cache->batch;
   p.heads = (int)heads;
   p.group = (int)(heads / cache->kv_heads);
-  p.head_tiles = d.head_tiles;
   p.max_length = (int)max_length;
-  p.chunk = d.chunk;
-  p.splits = d.splits;
   p.scaling = scaling;
-  hipStream_t st = (hipStream_t)stream;
-  const bool f16 = cache->dtype == MASE_DT_F16;
-  int lrc;
-  if (cache->head_dim == 64) lrc = launch_decode_d<64>(p, cache->format, f16, cache->batch, st);
-  else if (cache->head_dim == 128) lrc = launch_decode_d<128>(p, cache->format, f16, cache->batch, st);
-  else lrc = launch_decode_d<256>(p, cache->format, f16, cache->batch, st);
+  call.batch = cache->batch;
+  call.heads = heads;
+  call.kv_heads = cache->kv_heads;
+  call.max_length = max_length;
+  call.f16 = cache->dtype == MASE_DT_F16;
+  call.extra = mask != nullptr || weights != nullptr;
+  call.with_weights = weights != nullptr;
+  call.workspace = (unsigned char*)workspace;
+  call.workspace_bytes = workspace_bytes;
+  call.st = (hipStream_t)stream;
+  const int lrc = decode_dispatch(cache->head_dim, cache->format, call);
   if (lrc != MASE_OK) return lrc;
   return hipGetLastError() == hipSuccess ? MASE_OK : MASE_ERR_LAUNCH;
 }

@@ -251,10 +251,11 @@ def paged_attention_decode(query: Tensor, k_pages: Tensor, v_pages: Tensor, page
     out = torch.empty((batch, heads, head_dim), dtype=query.dtype, device=device)
     if batch == 0:
         return out
-    n = _bytes("mase_paged_attention_decode_workspace_bytes", device, batch, heads, kv_heads, head_dim, max_length, wp is not None)
-    ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
+    n = _bytes("mase_paged_attention_decode_workspace_bytes", device, batch, heads, kv_heads, head_dim, c.format, max_length,
+               wp is not None)
+    ws = torch.empty(n, dtype=torch.uint8, device=device)
     _call("mase_paged_attention_decode", device, ctypes.addressof(c), query.data_ptr(), *_strides(query), heads, lp, max_length,
-          float(scaling), mp, mcode, m_b, wp, w_b, w_h, out.data_ptr(), ws.data_ptr() if n else None, n)
+          float(scaling), mp, mcode, m_b, wp, w_b, w_h, out.data_ptr(), ws.data_ptr(), n)
     return out
 
 

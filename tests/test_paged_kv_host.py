@@ -131,9 +131,10 @@ def test_entry_points_refuse_bad_arguments(lib):
     assert decode(scaling=float("nan")) == -5 and decode(scaling=float("inf")) == -5
     assert decode(mask=p, mdt=2) == -4 and decode(q=p + 8) == -3 and decode(qs=(128, 60)) == -3 and decode(out=p + 8) == -3
     assert decode(w=p, ws=None, wsb=0) == -7 and decode(w=p, wsb=16) == -7 and decode(w=p, ws=p + 8) == -3
-    assert lib.mase_paged_attention_decode_workspace_bytes(1, 2, 2, 64, 16, 0) == 0  # one part: straight to the output
-    assert lib.mase_paged_attention_decode_workspace_bytes(1, 2, 2, 64, 16, 1) > 0
-    assert lib.mase_paged_attention_decode_workspace_bytes(1, 3, 2, 64, 16, 1) == 0
+    assert decode(ws=None, wsb=0) == -7 and decode(wsb=8) == -7
+    size = lib.mase_paged_attention_decode_workspace_bytes
+    assert 0 < size(1, 2, 2, 64, 0, 16, 0) < size(1, 2, 2, 64, 0, 16, 1)  # (batch, heads, kv_heads, head_dim, format, max_length, weights)
+    assert size(1, 3, 2, 64, 0, 16, 1) == 0 and size(1, 2, 2, 96, 0, 16, 1) == 0 and size(1, 2, 2, 64, 5, 16, 1) == 0
 
     def evict(**kw):
         d = dict(lengths=p, n=32, w=p, pos=p + 1024, cap=32, keep=8, recent=2, first=2, wo=p + 2048, po=p + 4096, lo=p, ws=p, wsb=1 << 16)
