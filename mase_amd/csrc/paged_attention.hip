@@ -14,24 +14,16 @@
 // MX codes are widened to 16 bits in registers as they are used (exact), two per conversion instruction for MXFP.
 #include "paged_kv.hpp"
 
-#ifndef MASE_PA_U8
-#define MASE_PA_U8 1
-#endif
-#ifndef MASE_PA_U4
-#define MASE_PA_U4 1
-#endif
-#ifndef MASE_PA_OCC
-#define MASE_PA_OCC 3
-#endif
-#ifndef MASE_PA_ROUNDS
-#define MASE_PA_ROUNDS 1
-#endif
 namespace mase {
 namespace {
 
 typedef __bf16 pa_bf16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 pa_f16x8_t __attribute__((ext_vector_type(8)));
 typedef float pa_f32x4_t __attribute__((ext_vector_type(4)));
+
+// int32 in memory that no kernel writes while this one runs: a uniform index reads it through the scalar cache, apart from
+// the vector loads in flight (which a vector load of a page number would have to wait for)
+typedef const __attribute__((address_space(4))) int32_t scalar_int;
 
 constexpr int kWaves = 4;
 constexpr int kHeadTile = 16;
@@ -44,7 +36,7 @@ struct DecodeParams {
   const int32_t* lengths;
   const unsigned char* mask;
   size_t mask_sb;  // elements
-  int mask_f32;
+  int mask_f32, mask_whole;  // mask_whole: four aligned values may be read at once
   unsigned char* out;
   unsigned long long* plan;  // [batch + 1] units of the sequences before (per row), then the units of a work-group
   float* part_o;    // [2 * work-groups][heads of a tile][D]
@@ -67,6 +59,13 @@ __device__ __forceinline__ pa_f32x4_t mfma16(const uint32_t* a, const uint32_t* 
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pa_bf16x8_t, av), __builtin_bit_cast(pa_bf16x8_t, bv), c, 0, 0, 0);
 }
 
+// low or high 16 bits of a word as a number
+template <bool F16>
+__device__ __forceinline__ float half_of(uint32_t w, int high) {
+  if constexpr (F16) return f16_bits_to_f32(high ? w >> 16 : w & 0xFFFFu);
+  return bits2f(high ? w & 0xFFFF0000u : w << 16);
+}
+
 // value of the lanes 16 apart and 32 apart combined
 __device__ __forceinline__ float max_over_groups(float v) {
   v = fmaxf(v, __shfl_xor(v, 16, 64));
@@ -78,9 +77,7 @@ __device__ __forceinline__ float sum_over_groups(float v) {
 }
 
 // How a format's rows are read.  Keys: lane group g of a row takes kRun consecutive elements per load, kKeyLoads loads
-// 4 kRun apart.  Values: a lane takes c = D / 16 consecutive elements of each of its 8 slots.  kU pairs of 16-slot tiles
-// make a wavefront's step: as many as hold about the bytes of one pair of 16-bit rows of 128 (what a wavefront has in
-// flight covers the latency of HBM).
+// 4 kRun apart.  Values: a lane takes c = D / 16 consecutive elements of each of its 8 slots.
 template <int D, int FMT>
 struct Rows {
   static constexpr int kBits = FMT == MASE_KV_16BIT ? 16 : (FMT == MASE_KV_MXFP4 ? 4 : 8);
@@ -93,10 +90,10 @@ struct Rows {
   static constexpr int kValWords = kValBytes < 4 ? 1 : kValBytes / 4;
   static constexpr bool kPacked = FMT != MASE_KV_16BIT;
   static constexpr int kScaleWords = kPacked ? (D == 256 ? 2 : 1) : 1;
-  static constexpr int kU = (D * kBits >= 2048) ? 1 : (D * kBits >= 1024 ? MASE_PA_U8 : MASE_PA_U4);
-  static constexpr int kSlots = 32 * kU;             // per wavefront and step
+  static constexpr int kSlots = 32;                 // per wavefront and step
   static constexpr int kUnit = kWaves * kSlots;      // per work-group and step
-  static constexpr int kPerCu = D == 256 ? (kPacked ? 2 : 1) : (D == 64 ? MASE_PA_OCC + 1 : MASE_PA_OCC);    // work-groups that a CU holds (registers)
+  // work-groups resident on a CU; see the comment on the kernel
+  static constexpr int kPerCu = D * kBits > 2048 ? 1 : 2;
 };
 
 // units (work-group steps) of a sequence's row; a sequence without a slot has one too, which writes its zeros
@@ -105,15 +102,15 @@ __device__ __forceinline__ int row_units(int length) {
   return length > 0 ? (length + UNIT - 1) / UNIT : 1;
 }
 
-// The rows (sequence, cached head, head tile) with their units in one line are cut into equal shares, one for each
-// work-group of the launch, all of them resident: sequences of any lengths keep every CU busy to the end.  A row that lies
-// in one share is finished by it; the pieces of a row that is cut go to the share's first or last place (2 wg, 2 wg + 1)
+// The sequences with their units in one line are cut into equal shares; a share is taken by one work-group for each (cached
+// head, head tile), all of them resident: sequences of any lengths keep every CU busy to the end, and the heads of a page,
+// which lie side by side in memory, are read at about the same time.  A row (sequence, cached head, head tile) that lies in
+// one share is finished by it; the pieces of a row that is cut go to the work-group's first or last place (2 wg, 2 wg + 1)
 // and are joined by the second kernel.
 // EXTRA: with a mask or weights.
 template <int D, int FMT, bool F16, bool EXTRA>
 __global__ __launch_bounds__(256, (Rows<D, FMT>::kPerCu)) void paged_decode_kernel(DecodeParams p) {
   using R = Rows<D, FMT>;
-  constexpr int kU = R::kU;
   constexpr float kGrow = F16 ? 4.0f : 8.0f;   // see the reference point of the exponentials below
   constexpr float kShift = F16 ? 11.0f : 0.0f;
   extern __shared__ __attribute__((aligned(16))) float lds[];
@@ -124,9 +121,12 @@ __global__ __launch_bounds__(256, (Rows<D, FMT>::kPerCu)) void paged_decode_kern
   const int i = lane & 15, g = lane >> 4;
   const int page_mask = (1 << p.c.page_shift) - 1;
   const int row_heads = p.c.heads * p.head_tiles;  // rows of a sequence
-  auto length_of = [&](int b) __attribute__((always_inline)) { return kv_length(p.lengths[b], p.max_length, p.c.table_pages, p.c.page_shift); };
+  const int rh = (int)blockIdx.x % row_heads, hk = rh / p.head_tiles, tile = rh % p.head_tiles;
+  const int rows = min(kHeadTile, p.group - tile * kHeadTile);  // query heads here
+  const int head0 = hk * p.group + tile * kHeadTile;
+  auto length_of = [&](int b) __attribute__((always_inline)) { return kv_length(((const scalar_int*)p.lengths)[b], p.max_length, p.c.table_pages, p.c.page_shift); };
 
-  // this work-group's share [u0, u1) of all units, and where it starts
+  // this work-group's share [u0, u1) of the units, and where it starts
   const int per = (p.batch + 255) / 256, b_lo = min((int)threadIdx.x * per, p.batch), b_hi = min(b_lo + per, p.batch);
   unsigned long long mine = 0;
   for (int b = b_lo; b < b_hi; ++b) mine += (unsigned)row_units<R::kUnit>(length_of(b));
@@ -144,9 +144,9 @@ __global__ __launch_bounds__(256, (Rows<D, FMT>::kPerCu)) void paged_decode_kern
     before += w < wave ? wave_sum[w] : 0ull;
     total += wave_sum[w];
   }
-  const unsigned long long units = total * (unsigned)row_heads;
-  const unsigned long long share = (units + gridDim.x - 1) / gridDim.x;
-  const unsigned long long u0 = share * blockIdx.x, u1 = min(u0 + share, units);
+  const unsigned shares = gridDim.x / (unsigned)row_heads;
+  const unsigned long long share = (total + shares - 1) / shares;
+  const unsigned long long u0 = share * (blockIdx.x / (unsigned)row_heads), u1 = min(u0 + share, total);
   if (blockIdx.x == 0) {
     unsigned long long at = before;
     for (int b = b_lo; b < b_hi; ++b) {
@@ -159,32 +159,29 @@ __global__ __launch_bounds__(256, (Rows<D, FMT>::kPerCu)) void paged_decode_kern
     }
   }
   if (u0 >= u1) return;
-  if (before * (unsigned)row_heads <= u0 && u0 < (before + mine) * (unsigned)row_heads) {  // one thread
-    unsigned long long at = before * (unsigned)row_heads;
+  if (before <= u0 && u0 < before + mine) {  // one thread
+    unsigned long long at = before;
     int b = b_lo;
     for (; b < b_hi - 1; ++b) {
-      const unsigned long long n = (unsigned long long)(unsigned)row_units<R::kUnit>(length_of(b)) * (unsigned)row_heads;
+      const unsigned long long n = (unsigned)row_units<R::kUnit>(length_of(b));
       if (u0 < at + n) break;
       at += n;
     }
     start_b = b;
-    start_at = (int)(u0 - at);  // below units of a row * rows: see the host's limit
+    start_at = (int)(u0 - at);
   }
   __syncthreads();
   int b = __builtin_amdgcn_readfirstlane(start_b);
+  int a = __builtin_amdgcn_readfirstlane(start_at);
   int length = length_of(b), n_units = row_units<R::kUnit>(length);
-  int rh = min(__builtin_amdgcn_readfirstlane(start_at) / n_units, row_heads - 1), a = __builtin_amdgcn_readfirstlane(start_at) % n_units;
   // units left, counted in 32 bits (the host's limit on the whole)
   int left = __builtin_amdgcn_readfirstlane((int)(u1 - u0));
 
 #pragma unroll 1
   for (bool first_piece = true;; first_piece = false) {
     const int e = min(n_units, a + left);  // this row's units a .. e - 1
-    const int hk = rh / p.head_tiles, tile = rh % p.head_tiles;
-    const int rows = min(kHeadTile, p.group - tile * kHeadTile);  // query heads here
-    const int head0 = hk * p.group + tile * kHeadTile;
     const int lo = a * R::kUnit, hi = min(e * R::kUnit, length);
-    const int32_t* table = p.c.table + (size_t)b * p.c.table_stride;
+    const scalar_int* table = (const scalar_int*)(p.c.table + (size_t)b * p.c.table_stride);
 
     uint32_t qf[D / 32][4];
 #pragma unroll
@@ -200,14 +197,17 @@ __global__ __launch_bounds__(256, (Rows<D, FMT>::kPerCu)) void paged_decode_kern
     // count as absent
     auto tile_page = [&](int slot, int& row) __attribute__((always_inline)) {
       row = slot & page_mask;
-      return slot < hi ? kv_page(table, p.c.table_pages, p.c.page_shift, p.c.num_pages, slot) : -1;
+      // (an entry that is there is read even if the slot is not: no branch)
+      const int at = min(slot >> p.c.page_shift, p.c.table_pages - 1);
+      const int pg = table[at];
+      return slot < hi && pg >= 0 && pg < p.c.num_pages ? pg : -1;
     };
-    uint32_t kr[2 * kU][R::kKeyLoads][R::kKeyWords], ksc[2 * kU][R::kScaleWords];
-    uint32_t vr[8 * kU][R::kValWords], vsc[2 * kU];
-    float mk[2 * kU][4];
+    uint32_t kr[2][R::kKeyLoads][R::kKeyWords], ksc[2][R::kScaleWords];
+    uint32_t vr[8][R::kValWords], vsc[2];
+    uint32_t mk[2][4];
     auto load_keys = [&](const int* page, const int* row) __attribute__((always_inline)) {
 #pragma unroll
-      for (int t = 0; t < 2 * kU; ++t) {
+      for (int t = 0; t < 2; ++t) {
         const int pg = max(page[t], 0);
         const unsigned char* base = p.c.k + (size_t)pg * p.c.k_page + (size_t)hk * p.c.k_head + (size_t)row[t] * p.c.k_slot;
 #pragma unroll
@@ -219,7 +219,7 @@ __global__ __launch_bounds__(256, (Rows<D, FMT>::kPerCu)) void paged_decode_kern
     };
     auto load_values = [&](const int* page, const int* row) __attribute__((always_inline)) {
 #pragma unroll
-      for (int t = 0; t < 2 * kU; ++t) {
+      for (int t = 0; t < 2; ++t) {
         const int pg = max(page[t], 0);
         const unsigned char* base = p.c.v + (size_t)pg * p.c.v_page + (size_t)hk * p.c.v_head + (size_t)row[t] * p.c.v_slot;
 #pragma unroll
@@ -229,17 +229,36 @@ __global__ __launch_bounds__(256, (Rows<D, FMT>::kPerCu)) void paged_decode_kern
           vsc[t] = *(const uint32_t*)(p.c.vs + (((((size_t)pg * p.c.heads + hk) * (D / 32)) + (i * R::kC) / 32) << p.c.page_shift) + row[t] + 4 * g);
       }
     };
-    // what is added to the scores of slots s0 + 16 t + 4 g + r (slots past the end read the last one's)
+    // what is added to the scores of slots s0 + 16 t + 4 g + r, as it lies in memory: one load of four where the mask's rows
+    // allow it; slots past the end read the last one's
     auto load_mask = [&](int s0) __attribute__((always_inline)) {
       if constexpr (EXTRA) {
         if (p.mask == nullptr) return;
+        const int size = p.mask_f32 ? 4 : 2;
+        const unsigned char* base = p.mask + (size_t)b * p.mask_sb * size;
+        if (p.mask_whole && s0 + R::kSlots <= hi) {
 #pragma unroll
-        for (int t = 0; t < 2 * kU; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const size_t at = (size_t)b * p.mask_sb + (size_t)min(s0 + 16 * t + 4 * g + r, hi - 1);
-            mk[t][r] = p.mask_f32 ? ((const float*)p.mask)[at] : DTypeTraits<F16 ? MASE_DT_F16 : MASE_DT_BF16>::load1(p.mask, at);
+          for (int t = 0; t < 2; ++t) {
+            const unsigned char* at = base + (size_t)(s0 + 16 * t + 4 * g) * size;
+            if (p.mask_f32) kv_load<16>(at, mk[t]);
+            else kv_load<8>(at, mk[t]);
           }
+        } else {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            size_t at[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) at[r] = (size_t)min(s0 + 16 * t + 4 * g + r, hi - 1);
+            if (p.mask_f32) {
+#pragma unroll
+              for (int r = 0; r < 4; ++r) mk[t][r] = ((const uint32_t*)base)[at[r]];
+            } else {
+              const uint16_t* h = (const uint16_t*)base;
+              mk[t][0] = h[at[0]] | ((uint32_t)h[at[1]] << 16);
+              mk[t][1] = h[at[2]] | ((uint32_t)h[at[3]] << 16);
+            }
+          }
+        }
       }
     };
 
@@ -252,24 +271,14 @@ __global__ __launch_bounds__(256, (Rows<D, FMT>::kPerCu)) void paged_decode_kern
     // scores: each overwrites the registers that were just used, so the loads need none of their own.  Page numbers are read
     // one step further ahead.  Past the end the last step's rows are read again (from the cache), which keeps the count of
     // loads in flight the same on every path.
-    int page[2 * kU], row[2 * kU], page_n[2 * kU], row_n[2 * kU];
+    int page[2], row[2], page_n[2], row_n[2];
     const int first = lo + wave * R::kSlots;
-    if (first < hi) {
-#pragma unroll
-      for (int t = 0; t < 2 * kU; ++t) {
-        page[t] = tile_page(first + 16 * t, row[t]);
-        page_n[t] = tile_page(first + R::kUnit + 16 * t, row_n[t]);
-      }
-      load_mask(first);
-      load_keys(page, row);
-      load_values(page, row);
-    }
-    for (int t0 = first; t0 < hi; t0 += R::kUnit) {
+    auto step = [&](int t0) __attribute__((always_inline)) {
       const bool more = t0 + R::kUnit < hi;
       // scores of head i at slots t0 + 16 t + 4 g + r
-      float x[2 * kU][4];
+      float x[2][4];
 #pragma unroll
-      for (int t = 0; t < 2 * kU; ++t) {
+      for (int t = 0; t < 2; ++t) {
         pa_f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int u = 0; u < R::kKeyLoads; ++u) {
@@ -286,50 +295,42 @@ __global__ __launch_bounds__(256, (Rows<D, FMT>::kPerCu)) void paged_decode_kern
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) x[t][r] = acc[r] * p.scaling;
-        if (kU > 1) __builtin_amdgcn_sched_barrier(0);
+        if (R::kPacked) __builtin_amdgcn_sched_barrier(0);
       }
-      bool whole = t0 + R::kSlots <= hi;
-#pragma unroll
-      for (int t = 0; t < 2 * kU; ++t) whole = whole && page[t] >= 0;
+      const bool some_gone = t0 + R::kSlots > hi || page[0] < 0 || page[1] < 0 || (EXTRA && p.mask != nullptr);  // perhaps
       uint32_t gone = 0;  // bit 4 t + r: the slot is absent
-      if (EXTRA && p.mask != nullptr) {
+      if (some_gone) {
 #pragma unroll
-        for (int t = 0; t < 2 * kU; ++t)
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            x[t][r] += mk[t][r];
-            if (mk[t][r] == -__builtin_inff()) gone |= 1u << (4 * t + r);
+            bool absent = page[t] < 0 || t0 + 16 * t + 4 * g + r >= hi;
+            if (EXTRA && p.mask != nullptr) {
+              const float add = p.mask_f32 ? bits2f(mk[t][r]) : half_of<F16>(mk[t][r >> 1], r & 1);
+              x[t][r] += add;
+              absent = absent || add == -__builtin_inff();
+            }
+            if (absent) {
+              x[t][r] = -__builtin_inff();
+              gone |= 1u << (4 * t + r);
+            }
           }
       }
-      if (!whole) {
 #pragma unroll
-        for (int t = 0; t < 2 * kU; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (page[t] < 0 || t0 + 16 * t + 4 * g + r >= hi) gone |= 1u << (4 * t + r);
-      }
-      if (EXTRA || !whole) {
-#pragma unroll
-        for (int t = 0; t < 2 * kU; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if ((gone >> (4 * t + r)) & 1u) x[t][r] = -__builtin_inff();
-      }
-#pragma unroll
-      for (int t = 0; t < 2 * kU; ++t) {  // the next step's pages, or the same again
+      for (int t = 0; t < 2; ++t) {  // the next step's pages, or the same again
         page[t] = more ? page_n[t] : page[t];
         row[t] = more ? row_n[t] : row[t];
       }
       load_mask(more ? t0 + R::kUnit : t0);
       load_keys(page, row);
 #pragma unroll
-      for (int t = 0; t < 2 * kU; ++t) page_n[t] = tile_page(t0 + 2 * R::kUnit + 16 * t, row_n[t]);
+      for (int t = 0; t < 2; ++t) page_n[t] = tile_page(t0 + 2 * R::kUnit + 16 * t, row_n[t]);
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (EXTRA) {
         if (p.scores != nullptr && i < rows) {
           float* sp = p.scores + ((size_t)b * p.heads + head0 + i) * p.score_stride + t0 + 4 * g;
 #pragma unroll
-          for (int t = 0; t < 2 * kU; ++t) *(float4*)(sp + 16 * t) = make_float4(x[t][0], x[t][1], x[t][2], x[t][3]);
+          for (int t = 0; t < 2; ++t) *(float4*)(sp + 16 * t) = make_float4(x[t][0], x[t][1], x[t][2], x[t][3]);
         }
       }
       // The reference point m of the exponentials moves only when some head has met a score more than kGrow (in the
@@ -337,7 +338,7 @@ __global__ __launch_bounds__(256, (Rows<D, FMT>::kPerCu)) void paged_decode_kern
       // between lanes.
       float mx = x[0][0];
 #pragma unroll
-      for (int t = 0; t < 2 * kU; ++t)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) mx = fmaxf(mx, x[t][r]);
       if (__builtin_amdgcn_ballot_w64((mx - m) * kLog2e > kGrow) != 0) {
@@ -349,8 +350,7 @@ __global__ __launch_bounds__(256, (Rows<D, FMT>::kPerCu)) void paged_decode_kern
         for (int n = 0; n < R::kC; ++n) o[n] *= alpha;
       }
       const float ms = m == -__builtin_inff() ? 0.0f : m;
-#pragma unroll
-      for (int u = 0; u < kU; ++u) {
+      {
         // fp16 probabilities are held 2^kShift up, where small ones keep their bits (fp16 loses them below 2^-14)
         uint32_t pf[4];
 #pragma unroll
@@ -358,38 +358,67 @@ __global__ __launch_bounds__(256, (Rows<D, FMT>::kPerCu)) void paged_decode_kern
           float ex[4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            ex[r] = __builtin_amdgcn_exp2f((x[2 * u + t][r] - ms) * kLog2e + kShift);
+            ex[r] = __builtin_amdgcn_exp2f((x[t][r] - ms) * kLog2e + kShift);
             l += ex[r];
           }
           pf[2 * t] = kv_pack2<F16>(ex[0], ex[1]);
           pf[2 * t + 1] = kv_pack2<F16>(ex[2], ex[3]);
         }
-        // values: widened slot by slot, then pairs of slots joined
-        uint32_t wv[8][R::kC / 2];
+        float vscale[8];
+        if constexpr (R::kPacked) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float scale = R::kPacked ? kv_scale<FMT>((vsc[2 * u + (j >> 2)] >> (8 * (j & 3))) & 0xFFu) : 0.0f;
-          kv_widen<FMT, F16, R::kC>(vr[8 * u + j], scale, wv[j]);
+          for (int j = 0; j < 8; ++j) vscale[j] = kv_scale<FMT>((vsc[j >> 2] >> (8 * (j & 3))) & 0xFFu);
         }
-        if (EXTRA || !whole) {  // what an absent slot holds must not meet its probability of zero: it may be infinite or NaN
+        if (some_gone) {  // what an absent slot holds must not meet its probability of zero: it may be infinite or NaN
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            if ((gone >> (8 * u + j)) & 1u) {
+            if ((gone >> j) & 1u) {
+              if constexpr (R::kPacked) vscale[j] = 0.0f;
 #pragma unroll
-              for (int n = 0; n < R::kC / 2; ++n) wv[j][n] = 0;
+              for (int n = 0; n < R::kValWords; ++n) vr[j][n] = 0;
             }
         }
+        // values: two neighbouring elements of the 8 slots at a time, widened, pairs of slots joined
 #pragma unroll
-        for (int n = 0; n < R::kC; ++n) {
-          uint32_t f[4];
+        for (int np = 0; np < R::kC / 2; ++np) {
+          uint32_t f0[4], f1[4];
+          if constexpr (FMT == MASE_KV_MXINT8) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) f[q] = __builtin_amdgcn_perm(wv[2 * q + 1][n >> 1], wv[2 * q][n >> 1], (n & 1) ? 0x07060302u : 0x05040100u);
-          o[n] = mfma16<F16>(f, pf, o[n]);
+            for (int q = 0; q < 4; ++q) {
+              const uint32_t wa = vr[2 * q][np >> 1] >> (16 * (np & 1)), wb = vr[2 * q + 1][np >> 1] >> (16 * (np & 1));
+              f0[q] = kv_pack2<F16>((float)(int)(int8_t)wa * vscale[2 * q], (float)(int)(int8_t)wb * vscale[2 * q + 1]);
+              f1[q] = kv_pack2<F16>((float)(int)(int8_t)(wa >> 8) * vscale[2 * q], (float)(int)(int8_t)(wb >> 8) * vscale[2 * q + 1]);
+            }
+          } else {
+            uint32_t w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = kv_widen_pair<FMT, F16>(vr[j], np, R::kPacked ? vscale[j] : 0.0f);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              f0[q] = __builtin_amdgcn_perm(w[2 * q + 1], w[2 * q], 0x05040100u);
+              f1[q] = __builtin_amdgcn_perm(w[2 * q + 1], w[2 * q], 0x07060302u);
+            }
+          }
+          o[2 * np] = mfma16<F16>(f0, pf, o[2 * np]);
+          o[2 * np + 1] = mfma16<F16>(f1, pf, o[2 * np + 1]);
+          if (R::kPacked && (np & 1)) __builtin_amdgcn_sched_barrier(0);
         }
-        if (kU > 1) __builtin_amdgcn_sched_barrier(0);
       }
       load_values(page, row);
       __builtin_amdgcn_sched_barrier(0);
+    };
+    if (first < hi) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        page[t] = tile_page(first + 16 * t, row[t]);
+        page_n[t] = tile_page(first + R::kUnit + 16 * t, row_n[t]);
+      }
+      load_mask(first);
+      load_keys(page, row);
+      __builtin_amdgcn_sched_barrier(0);  // the order of the loop, which its waits count on
+      load_values(page, row);
+      __builtin_amdgcn_sched_barrier(0);
+      for (int t0 = first; t0 < hi; t0 += R::kUnit) step(t0);
     }
 
     // join the wavefronts: [wave][head] maxima and sums, [wave][head][D] outputs
@@ -446,29 +475,26 @@ __global__ __launch_bounds__(256, (Rows<D, FMT>::kPerCu)) void paged_decode_kern
     if (left <= 0) break;
     __syncthreads();  // everyone has read the LDS
     a = 0;
-    if (++rh == row_heads) {
-      rh = 0;
-      if (++b >= p.batch) break;  // lengths that change under the kernel must not lead past the last sequence
-      length = length_of(b);
-      n_units = row_units<R::kUnit>(length);
-    }
+    if (++b >= p.batch) break;  // lengths that change under the kernel must not lead past the last sequence
+    length = length_of(b);
+    n_units = row_units<R::kUnit>(length);
   }
 }
 
 // The pieces of row `rh` of sequence b: how many (1: the row was finished in one piece), and where piece k lies.
 struct Pieces {
-  int count;
-  unsigned long long wg0;
+  int count, row_heads;
+  size_t wg0;  // the first piece's work-group; the next ones' are row_heads apart
   bool from_start;
-  __device__ __forceinline__ size_t place(int k) const { return 2 * (size_t)(wg0 + k) + (k == 0 && !from_start ? 1 : 0); }
+  __device__ __forceinline__ size_t place(int k) const { return 2 * (wg0 + (size_t)k * row_heads) + (k == 0 && !from_start ? 1 : 0); }
 };
 __device__ __forceinline__ Pieces row_pieces(const DecodeParams& p, int b, int rh, int row_heads) {
-  const unsigned long long before = p.plan[b], n = p.plan[b + 1] - before, share = p.plan[p.batch + 1];
-  const unsigned long long at = before * (unsigned)row_heads + (unsigned long long)rh * n;
+  const unsigned long long at = p.plan[b], n = p.plan[b + 1] - at, share = p.plan[p.batch + 1], s0 = at / share;
   Pieces q;
-  q.wg0 = at / share;
-  q.from_start = q.wg0 * share == at;
-  q.count = (int)((at + n - 1) / share - q.wg0) + 1;
+  q.row_heads = row_heads;
+  q.wg0 = (size_t)s0 * row_heads + rh;
+  q.from_start = s0 * share == at;
+  q.count = (int)((at + n - 1) / share - s0) + 1;
   return q;
 }
 
@@ -566,7 +592,7 @@ __global__ __launch_bounds__(256) void paged_decode_join_kernel(DecodeParams p, 
 
 // What a call launches and keeps between its two kernels.
 struct DecodePlan {
-  int groups;      // work-groups
+  size_t groups;   // work-groups
   int head_tiles, tile_rows;
   bool join;       // a row may be cut
   size_t score_stride, plan_bytes, part_floats, ml_floats, row_ml_floats, score_floats;
@@ -583,13 +609,16 @@ DecodePlan decode_plan(size_t batch, size_t heads, size_t kv_heads, size_t max_l
   int cus = device_cu_count();
   if (cus <= 0) cus = 256;
   const size_t steps = max_length ? (max_length + R::kUnit - 1) / R::kUnit : 1;
-  const size_t most = batch * kv_heads * d.head_tiles * steps;
-  d.groups = (int)(most < (size_t)cus * R::kPerCu * MASE_PA_ROUNDS ? most : (size_t)cus * R::kPerCu * MASE_PA_ROUNDS);
+  const size_t row_heads = kv_heads * d.head_tiles, resident = (size_t)cus * R::kPerCu;
+  size_t shares = resident / row_heads;
+  if (shares < 1) shares = 1;
+  if (shares > batch * steps) shares = batch * steps;
+  d.groups = shares * row_heads;
   d.join = steps > 1;
   d.score_stride = steps * R::kUnit;
   d.plan_bytes = (batch + 2 + 1) / 2 * 2 * sizeof(unsigned long long);
-  d.part_floats = d.join ? 2 * (size_t)d.groups * d.tile_rows * D : 0;
-  d.ml_floats = d.join ? 2 * (size_t)d.groups * d.tile_rows * 2 : 0;
+  d.part_floats = d.join ? 2 * d.groups * d.tile_rows * D : 0;
+  d.ml_floats = d.join ? 2 * d.groups * d.tile_rows * 2 : 0;
   d.row_ml_floats = weights ? (batch * heads * 2 + 3) / 4 * 4 : 0;
   d.score_floats = weights ? batch * heads * d.score_stride : 0;
   return d;
@@ -597,10 +626,15 @@ DecodePlan decode_plan(size_t batch, size_t heads, size_t kv_heads, size_t max_l
 
 template <int D, int FMT, bool F16, bool EXTRA>
 int launch_decode(const DecodeParams& p, const DecodePlan& d, hipStream_t st) {
-  const size_t lds = sizeof(float) * (2 * kWaves * kHeadTile + (size_t)kWaves * d.tile_rows * D);
+  // as much LDS as lets exactly kPerCu work-groups on a CU: where one more would fit, some CUs take it and others are left
+  // with one less, and the launch lasts as long as the fullest CU
+  constexpr size_t kLdsCu = 160 * 1024, kOnly = kLdsCu / (Rows<D, FMT>::kPerCu + 1) + 64;
+  constexpr size_t kMost = sizeof(float) * (2 * kWaves * kHeadTile + kWaves * kHeadTile * D);
+  static_assert(kMost + 256 <= kLdsCu / Rows<D, FMT>::kPerCu && kOnly + 256 <= kLdsCu / Rows<D, FMT>::kPerCu, "kPerCu work-groups fit");
+  const size_t need = sizeof(float) * (2 * kWaves * kHeadTile + (size_t)kWaves * d.tile_rows * D), lds = need > kOnly ? need : kOnly;
   static std::atomic<uint64_t> attr_done{0};
   const void* fn = (const void*)paged_decode_kernel<D, FMT, F16, EXTRA>;
-  if (!set_dynamic_lds_once(attr_done, fn, (int)sizeof(float) * (2 * kWaves * kHeadTile + kWaves * kHeadTile * D))) return MASE_ERR_LAUNCH;
+  if (!set_dynamic_lds_once(attr_done, fn, (int)(kMost > kOnly ? kMost : kOnly))) return MASE_ERR_LAUNCH;
   hipLaunchKernelGGL((paged_decode_kernel<D, FMT, F16, EXTRA>), dim3((unsigned)d.groups), dim3(256), lds, st, p);
   const bool weights = p.scores != nullptr;
   if (!d.join && !weights) return MASE_OK;
@@ -630,9 +664,9 @@ int decode_call(DecodeCall& c) {
   }
   if (c.workspace == nullptr || c.workspace_bytes < d.bytes()) return MASE_ERR_WORKSPACE;
   if (!aligned16(c.workspace)) return MASE_ERR_ALIGN;
-  // a place within one sequence's rows, and a work-group's share with a row's units on top, are counted in 32 bits
-  const size_t row = c.max_length / Rows<D, FMT>::kUnit + 1, rows = c.kv_heads * d.head_tiles;
-  if (row * rows > 0x3FFFFFFFu || c.batch * rows * row / (size_t)d.groups > 0x3FFFFFFEu) return MASE_ERR_SHAPE;
+  // a work-group's share with a row's units on top is counted in 32 bits
+  const size_t row = c.max_length / Rows<D, FMT>::kUnit + 1;
+  if (row * c.batch > 0x3FFFFFFFu || d.groups > 0x7FFFFFFFu) return MASE_ERR_SHAPE;
   c.p.plan = (unsigned long long*)c.workspace;
   float* f = (float*)(c.workspace + d.plan_bytes);
   c.p.part_o = f;
@@ -706,6 +740,7 @@ extern "C" int mase_paged_attention_decode(const mase_paged_kv* cache, const voi
   p.mask = (const unsigned char*)mask;
   p.mask_sb = mask_stride_b;
   p.mask_f32 = mask_dtype == MASE_DT_F32;
+  p.mask_whole = mask_stride_b % 4 == 0 && ((uintptr_t)mask & (p.mask_f32 ? 15u : 7u)) == 0;
   p.out = (unsigned char*)out;
   p.weights = weights;
   p.w_sb = w_stride_b;

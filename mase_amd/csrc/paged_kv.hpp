@@ -91,6 +91,23 @@ __device__ __forceinline__ void kv_widen(const uint32_t* w, float scale, uint32_
   }
 }
 
+// elements 2 np and 2 np + 1 of a run in its storage words
+template <int FMT, bool F16>
+__device__ __forceinline__ uint32_t kv_widen_pair(const uint32_t* w, int np, float scale) {
+  if constexpr (FMT == MASE_KV_16BIT) {
+    return w[np];
+  } else if constexpr (FMT == MASE_KV_MXFP4) {
+    switch (np & 3) {
+      case 0: return kv_widen2<FMT, F16, 0>(w[np >> 2], scale);
+      case 1: return kv_widen2<FMT, F16, 1>(w[np >> 2], scale);
+      case 2: return kv_widen2<FMT, F16, 2>(w[np >> 2], scale);
+      default: return kv_widen2<FMT, F16, 3>(w[np >> 2], scale);
+    }
+  } else {
+    return (np & 1) ? kv_widen2<FMT, F16, 1>(w[np >> 1], scale) : kv_widen2<FMT, F16, 0>(w[np >> 1], scale);
+  }
+}
+
 // BYTES (2 .. 32) from memory to words; a 2-byte piece fills the low half of one word
 template <int BYTES>
 __device__ __forceinline__ void kv_load(const unsigned char* p, uint32_t* w) {
