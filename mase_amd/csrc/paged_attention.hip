@@ -38,7 +38,7 @@ struct DecodeParams {
   size_t mask_sb;  // elements
   int mask_f32, mask_whole;  // mask_whole: four aligned values may be read at once
   unsigned char* out;
-  unsigned long long* plan;  // [batch + 1] units of the sequences before (per row), then the units of a work-group
+  uint32_t* plan;  // [batch + 1] units of the sequences before each, then the units of a share
   float* part_o;    // [2 * work-groups][heads of a tile][D]
   float* part_ml;   // [2 * work-groups][heads of a tile][2]
   float* row_ml;    // [batch * heads][2], with weights
@@ -114,7 +114,7 @@ __global__ __launch_bounds__(256, (Rows<D, FMT>::kPerCu)) void paged_decode_kern
   constexpr float kGrow = F16 ? 4.0f : 8.0f;   // see the reference point of the exponentials below
   constexpr float kShift = F16 ? 11.0f : 0.0f;
   extern __shared__ __attribute__((aligned(16))) float lds[];
-  __shared__ unsigned long long wave_sum[kWaves];
+  __shared__ uint32_t wave_sum[kWaves];
   __shared__ int start_b, start_at;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -126,29 +126,29 @@ __global__ __launch_bounds__(256, (Rows<D, FMT>::kPerCu)) void paged_decode_kern
   const int head0 = hk * p.group + tile * kHeadTile;
   auto length_of = [&](int b) __attribute__((always_inline)) { return kv_length(((const scalar_int*)p.lengths)[b], p.max_length, p.c.table_pages, p.c.page_shift); };
 
-  // this work-group's share [u0, u1) of the units, and where it starts
+  // this work-group's share [u0, u1) of the units (32 bits: the host's limit), and where it starts
   const int per = (p.batch + 255) / 256, b_lo = min((int)threadIdx.x * per, p.batch), b_hi = min(b_lo + per, p.batch);
-  unsigned long long mine = 0;
+  uint32_t mine = 0;
   for (int b = b_lo; b < b_hi; ++b) mine += (unsigned)row_units<R::kUnit>(length_of(b));
-  unsigned long long run = mine;
+  uint32_t run = mine;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
-    const unsigned long long o = __shfl_up(run, d, 64);
+    const uint32_t o = __shfl_up(run, d, 64);
     if (lane >= d) run += o;
   }
   if (lane == 63) wave_sum[wave] = run;
   __syncthreads();
-  unsigned long long before = run - mine, total = 0;
+  uint32_t before = run - mine, total = 0;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
-    before += w < wave ? wave_sum[w] : 0ull;
+    before += w < wave ? wave_sum[w] : 0u;
     total += wave_sum[w];
   }
   const unsigned shares = gridDim.x / (unsigned)row_heads;
-  const unsigned long long share = (total + shares - 1) / shares;
-  const unsigned long long u0 = share * (blockIdx.x / (unsigned)row_heads), u1 = min(u0 + share, total);
+  const uint32_t share = (total + shares - 1) / shares;
+  const uint32_t u0 = min(share * (blockIdx.x / (unsigned)row_heads), total), u1 = min(u0 + share, total);
   if (blockIdx.x == 0) {
-    unsigned long long at = before;
+    uint32_t at = before;
     for (int b = b_lo; b < b_hi; ++b) {
       p.plan[b] = at;
       at += (unsigned)row_units<R::kUnit>(length_of(b));
@@ -160,10 +160,10 @@ __global__ __launch_bounds__(256, (Rows<D, FMT>::kPerCu)) void paged_decode_kern
   }
   if (u0 >= u1) return;
   if (before <= u0 && u0 < before + mine) {  // one thread
-    unsigned long long at = before;
+    uint32_t at = before;
     int b = b_lo;
     for (; b < b_hi - 1; ++b) {
-      const unsigned long long n = (unsigned)row_units<R::kUnit>(length_of(b));
+      const uint32_t n = (unsigned)row_units<R::kUnit>(length_of(b));
       if (u0 < at + n) break;
       at += n;
     }
@@ -174,7 +174,6 @@ __global__ __launch_bounds__(256, (Rows<D, FMT>::kPerCu)) void paged_decode_kern
   int b = __builtin_amdgcn_readfirstlane(start_b);
   int a = __builtin_amdgcn_readfirstlane(start_at);
   int length = length_of(b), n_units = row_units<R::kUnit>(length);
-  // units left, counted in 32 bits (the host's limit on the whole)
   int left = __builtin_amdgcn_readfirstlane((int)(u1 - u0));
 
 #pragma unroll 1
@@ -489,7 +488,7 @@ struct Pieces {
   __device__ __forceinline__ size_t place(int k) const { return 2 * (wg0 + (size_t)k * row_heads) + (k == 0 && !from_start ? 1 : 0); }
 };
 __device__ __forceinline__ Pieces row_pieces(const DecodeParams& p, int b, int rh, int row_heads) {
-  const unsigned long long at = p.plan[b], n = p.plan[b + 1] - at, share = p.plan[p.batch + 1], s0 = at / share;
+  const uint32_t at = p.plan[b], n = p.plan[b + 1] - at, share = p.plan[p.batch + 1], s0 = at / share;
   Pieces q;
   q.row_heads = row_heads;
   q.wg0 = (size_t)s0 * row_heads + rh;
@@ -498,79 +497,83 @@ __device__ __forceinline__ Pieces row_pieces(const DecodeParams& p, int b, int r
   return q;
 }
 
-// max and sum over the pieces of one head, by one wavefront
-__device__ __forceinline__ void head_ml(const DecodeParams& p, const Pieces& q, int r, int lane, float& top, float& sum) {
-  top = -__builtin_inff();
-  for (int k = lane; k < q.count; k += 64) top = fmaxf(top, p.part_ml[(q.place(k) * p.tile_rows + r) * 2]);
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-  sum = 0.0f;
-  for (int k = lane; k < q.count; k += 64) {
-    const float* ml = p.part_ml + (q.place(k) * p.tile_rows + r) * 2;
-    sum += ml[1] * (ml[0] == top ? 1.0f : __builtin_amdgcn_exp2f((ml[0] - top) * kLog2e));
-  }
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
+// A running softmax: reference point, sum of exponentials, and (joining) their weighted sum.  Later terms are added with one
+// rescaling at most; NaN stays.
+__device__ __forceinline__ void ml_add(float& top, float& sum, float4& acc, float m, float l, const float4& v) {
+  const float t = fmaxf(top, m);
+  const float f = top == t ? 1.0f : __builtin_amdgcn_exp2f((top - t) * kLog2e), g = m == t ? 1.0f : __builtin_amdgcn_exp2f((m - t) * kLog2e);
+  top = t;
+  sum = sum * f + l * g;
+  acc.x = acc.x * f + v.x * g;
+  acc.y = acc.y * f + v.y * g;
+  acc.z = acc.z * f + v.z * g;
+  acc.w = acc.w * f + v.w * g;
 }
 
 constexpr int kMaxGroup = 256;
 constexpr int kWeightSlots = 1024;  // per work-group
-constexpr int kJoinCols = 32;       // of the head dimension per work-group
 
-// Joins the pieces of cut rows (blocks x < joins: one query head of the cached head and kJoinCols columns each) and, with
-// weights, adds the probabilities of kWeightSlots slots (the blocks behind).  grid (x, cached head, sequence).
+// Joins the pieces of cut rows.  grid (x, row, sequence): a work-group takes `items` (a power of two from 16 to 256) of the
+// row's rows * D / 4 groups of four outputs, 256 / items threads sharing the pieces of each; the host takes as few items as
+// make 256 work-groups of all rows.  The pieces' sums are added in a fixed order.
 template <int D, bool F16>
-__global__ __launch_bounds__(256) void paged_decode_join_kernel(DecodeParams p, int joins) {
+__global__ __launch_bounds__(256) void paged_decode_join_kernel(DecodeParams p, int items) {
+  __shared__ __attribute__((aligned(16))) float4 acc_s[256];
+  __shared__ float top_s[256], sum_s[256];
+  const int rh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+  const int row_heads = p.c.heads * p.head_tiles;
+  const Pieces q = row_pieces(p, b, rh, row_heads);
+  if (q.count == 1) return;
+  const int hk = rh / p.head_tiles, tile = rh % p.head_tiles;
+  const int rows = min(kHeadTile, p.group - tile * kHeadTile);
+  const int item = (int)blockIdx.x * items + tid % items, r = item / (D / 4), col = item % (D / 4) * 4;
+  const int parts = 256 / items;
+  float top = -__builtin_inff(), sum = 0.0f;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (r < rows) {
+#pragma unroll 4
+    for (int k = tid / items; k < q.count; k += parts) {
+      const size_t place = q.place(k) * p.tile_rows + r;
+      const float2 ml = *(const float2*)(p.part_ml + place * 2);
+      ml_add(top, sum, acc, ml.x, ml.y, *(const float4*)(p.part_o + place * D + col));
+    }
+  }
+  acc_s[tid] = acc;
+  top_s[tid] = top;
+  sum_s[tid] = sum;
+  __syncthreads();
+  if (tid >= items || r >= rows) return;
+  for (int k = 1; k < parts; ++k) ml_add(top, sum, acc, top_s[k * items + tid], sum_s[k * items + tid], acc_s[k * items + tid]);
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const size_t bh = (size_t)b * p.heads + hk * p.group + tile * kHeadTile + r;
+  uint2 y;
+  y.x = kv_pack2<F16>(acc.x * inv, acc.y * inv);
+  y.y = kv_pack2<F16>(acc.z * inv, acc.w * inv);
+  *(uint2*)(p.out + (bh * D + col) * 2) = y;
+}
+
+// Adds the probabilities of kWeightSlots slots, summed over the query heads of a cached head, to the weights.
+// grid (share of the slots, cached head, sequence).
+__global__ __launch_bounds__(256) void paged_decode_weights_kernel(DecodeParams p) {
   __shared__ float top_s[kMaxGroup], inv_s[kMaxGroup];
-  __shared__ __attribute__((aligned(16))) float red[256 * 4];
   const int hk = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int row_heads = p.c.heads * p.head_tiles;
   const size_t bh0 = (size_t)b * p.heads + (size_t)hk * p.group;
-  if ((int)blockIdx.x < joins) {
-    const int h = (int)blockIdx.x / (D / kJoinCols), col0 = ((int)blockIdx.x % (D / kJoinCols)) * kJoinCols;
-    const Pieces q = row_pieces(p, b, hk * p.head_tiles + h / kHeadTile, row_heads);
-    if (q.count == 1) return;
-    const int r = h % kHeadTile;
-    float top, sum;
-    head_ml(p, q, r, lane, top, sum);  // every wavefront for itself
-    constexpr int kCols = kJoinCols / 4, kRows = 256 / kCols;  // threads along the columns, pieces side by side
-    const int col = tid % kCols, at = tid / kCols;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-    for (int k = at; k < q.count; k += kRows) {
-      const size_t place = q.place(k) * p.tile_rows + r;
-      const float mk = p.part_ml[place * 2];
-      const float4 v = *(const float4*)(p.part_o + place * D + col0 + col * 4);
-      const float f = mk == top ? 1.0f : __builtin_amdgcn_exp2f((mk - top) * kLog2e);
-      acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
-    }
-    ((float4*)red)[tid] = acc;
-    __syncthreads();
-    if (tid < kCols) {
-      for (int k = 1; k < kRows; ++k) {
-        const float4 v = ((const float4*)red)[k * kCols + tid];
-        acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
-      }
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      uint2 y;
-      y.x = kv_pack2<F16>(acc.x * inv, acc.y * inv);
-      y.y = kv_pack2<F16>(acc.z * inv, acc.w * inv);
-      *(uint2*)(p.out + ((bh0 + h) * D + col0 + tid * 4) * 2) = y;
-    }
-    return;
-  }
-  const int s0 = ((int)blockIdx.x - joins) * kWeightSlots;
+  const int s0 = (int)blockIdx.x * kWeightSlots;
   const int length = kv_length(p.lengths[b], p.max_length, p.c.table_pages, p.c.page_shift);
   if (s0 >= length) return;
   for (int h = wave; h < p.group; h += 4) {
     const Pieces q = row_pieces(p, b, hk * p.head_tiles + h / kHeadTile, row_heads);
-    float top, sum;
-    if (q.count == 1) {
-      top = p.row_ml[(bh0 + h) * 2];
-      sum = p.row_ml[(bh0 + h) * 2 + 1];
-    } else {
-      head_ml(p, q, h % kHeadTile, lane, top, sum);
+    float top = -__builtin_inff(), sum = 0.0f;
+    float4 none = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const float4 zero = none;
+    for (int k = lane; k < q.count; k += 64) {
+      const float2 ml = q.count == 1 ? *(const float2*)(p.row_ml + (bh0 + h) * 2)
+                                     : *(const float2*)(p.part_ml + (q.place(k) * p.tile_rows + h % kHeadTile) * 2);
+      ml_add(top, sum, none, ml.x, ml.y, zero);
     }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) ml_add(top, sum, none, __shfl_xor(top, d, 64), __shfl_xor(sum, d, 64), zero);
     if (lane == 0) {
       top_s[h] = top;
       inv_s[h] = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -578,15 +581,23 @@ __global__ __launch_bounds__(256) void paged_decode_join_kernel(DecodeParams p, 
   }
   __syncthreads();
   float* wrow = p.weights + (size_t)b * p.w_sb + (size_t)hk * p.w_sh;
-  const int end = min(length, s0 + kWeightSlots);
-  for (int s = s0 + tid; s < end; s += 256) {
-    float acc = 0.0f;
-    for (int h = 0; h < p.group; ++h) {
-      const float x = p.scores[(bh0 + h) * p.score_stride + s];
-      const float e = x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((x - top_s[h]) * kLog2e);
-      acc += e * inv_s[h];
+  float acc[kWeightSlots / 256];
+#pragma unroll
+  for (int j = 0; j < kWeightSlots / 256; ++j) acc[j] = 0.0f;
+  const int last = length - 1;
+  for (int h = 0; h < p.group; ++h) {
+    const float* xs = p.scores + (bh0 + h) * p.score_stride;
+    const float top = top_s[h], inv = inv_s[h];
+#pragma unroll
+    for (int j = 0; j < kWeightSlots / 256; ++j) {
+      const float x = xs[min(s0 + 256 * j + tid, last)];
+      acc[j] += (x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((x - top) * kLog2e)) * inv;
     }
-    wrow[s] += acc;
+  }
+#pragma unroll
+  for (int j = 0; j < kWeightSlots / 256; ++j) {
+    const int s = s0 + 256 * j + tid;
+    if (s < length) wrow[s] += acc[j];
   }
 }
 
@@ -616,7 +627,7 @@ DecodePlan decode_plan(size_t batch, size_t heads, size_t kv_heads, size_t max_l
   d.groups = shares * row_heads;
   d.join = steps > 1;
   d.score_stride = steps * R::kUnit;
-  d.plan_bytes = (batch + 2 + 1) / 2 * 2 * sizeof(unsigned long long);
+  d.plan_bytes = (batch + 2 + 3) / 4 * 4 * sizeof(uint32_t);
   d.part_floats = d.join ? 2 * d.groups * d.tile_rows * D : 0;
   d.ml_floats = d.join ? 2 * d.groups * d.tile_rows * 2 : 0;
   d.row_ml_floats = weights ? (batch * heads * 2 + 3) / 4 * 4 : 0;
@@ -636,12 +647,14 @@ int launch_decode(const DecodeParams& p, const DecodePlan& d, hipStream_t st) {
   const void* fn = (const void*)paged_decode_kernel<D, FMT, F16, EXTRA>;
   if (!set_dynamic_lds_once(attr_done, fn, (int)(kMost > kOnly ? kMost : kOnly))) return MASE_ERR_LAUNCH;
   hipLaunchKernelGGL((paged_decode_kernel<D, FMT, F16, EXTRA>), dim3((unsigned)d.groups), dim3(256), lds, st, p);
-  const bool weights = p.scores != nullptr;
-  if (!d.join && !weights) return MASE_OK;
-  const unsigned joins = d.join ? (unsigned)(p.group * (D / kJoinCols)) : 0;
-  const unsigned shares = weights ? blocks_for((size_t)p.max_length, kWeightSlots) : 0;
-  if (joins + shares > 0)
-    hipLaunchKernelGGL((paged_decode_join_kernel<D, F16>), dim3(joins + shares, (unsigned)p.c.heads, (unsigned)p.batch), dim3(256), 0, st, p, (int)joins);
+  if (d.join) {
+    const size_t rows = (size_t)p.c.heads * d.head_tiles, all = (size_t)d.tile_rows * (D / 4);
+    int items = 256;
+    while (items > 16 && ((size_t)items / 2 >= all || (size_t)p.batch * rows * ((all + items - 1) / items) < 256)) items /= 2;
+    hipLaunchKernelGGL((paged_decode_join_kernel<D, F16>), dim3(blocks_for(all, (size_t)items), (unsigned)rows, (unsigned)p.batch), dim3(256), 0, st, p, items);
+  }
+  if (EXTRA && p.scores != nullptr && p.max_length > 0)
+    hipLaunchKernelGGL(paged_decode_weights_kernel, dim3(blocks_for((size_t)p.max_length, kWeightSlots), (unsigned)p.c.heads, (unsigned)p.batch), dim3(256), 0, st, p);
   return MASE_OK;
 }
 
@@ -664,10 +677,10 @@ int decode_call(DecodeCall& c) {
   }
   if (c.workspace == nullptr || c.workspace_bytes < d.bytes()) return MASE_ERR_WORKSPACE;
   if (!aligned16(c.workspace)) return MASE_ERR_ALIGN;
-  // a work-group's share with a row's units on top is counted in 32 bits
+  // units are counted in 32 bits: all of them, rounded up to whole shares, and a share with a row's on top
   const size_t row = c.max_length / Rows<D, FMT>::kUnit + 1;
   if (row * c.batch > 0x3FFFFFFFu || d.groups > 0x7FFFFFFFu) return MASE_ERR_SHAPE;
-  c.p.plan = (unsigned long long*)c.workspace;
+  c.p.plan = (uint32_t*)c.workspace;
   float* f = (float*)(c.workspace + d.plan_bytes);
   c.p.part_o = f;
   c.p.part_ml = f + d.part_floats;
