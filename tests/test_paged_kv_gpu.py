@@ -295,6 +295,28 @@ def test_decode_one_mask_row_for_all(dev):
     check_decode(dev, p, 4, 18, mask=torch.randn(1, 128, generator=gen(19)))
 
 
+@pytest.mark.parametrize("mask_dtype", ["own", torch.float32])
+@pytest.mark.parametrize("n,offset,stride", [(1, 0, 1), (2, 1, 5), (3, 0, 3), (4, 3, 7), (5, 1, 6), (130, 1, 131), (257, 2, 263)])
+def test_decode_mask_rows_of_any_alignment(dev, n, offset, stride, mask_dtype):
+    """masks that end with the last slot, start at any element and have odd strides; short ones"""
+    p = Pool(gen(60), [n, max(1, n - 1)], 2, 128, 16, "mxfp8_e5m2" if n % 2 else None, torch.bfloat16)
+    mt = torch.bfloat16 if mask_dtype == "own" else mask_dtype
+    flat = torch.full((offset + stride + n,), math.nan, dtype=mt)  # what lies around the rows is never added
+    mask = flat.as_strided((2, n), (stride, 1), offset)
+    mask.copy_(torch.randn(2, n, generator=gen(61)))
+    check = flat.to(dev)
+    g = gen(62)
+    q = torch.randn(2, 8, 128, generator=g).bfloat16()
+    w = torch.zeros(2, 2, p.table.shape[1] * 16, device=dev)
+    out = F().paged_attention_decode(q.to(dev), **p.to(dev), lengths=i32(p.lengths, dev), max_length=n,
+                                     mask=check.as_strided((2, n), (stride, 1), offset), weights=w).cpu()
+    for i, m in enumerate(p.lengths):
+        k, v = p.rows(i, m)
+        o, pr, to, tp = attend(q[i], k, v, 128 ** -0.5, mask[i, :m].double(), torch.bfloat16)
+        assert bool(((out[i].double() - o).abs() <= to).all())
+        assert bool(((w[i, :, :m].cpu().double() - pr.view(2, 4, m).sum(1)).abs() <= tp.view(2, 4, m).sum(1) + 5 * HALF[torch.float32]).all())
+
+
 @pytest.mark.parametrize("scaling", [0.0, -0.2, 3.0])
 def test_decode_scalings(dev, scaling):
     p = Pool(gen(20), [200, 77], 2, 64, 16, None, torch.bfloat16)
