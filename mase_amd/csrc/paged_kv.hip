@@ -203,21 +203,19 @@ struct GatherParams {
   int max_length;
 };
 
-// 16 elements (codes) or 8 (16-bit rows) of keys and of values per lane
+// 8 elements of keys and of values per lane: a store instruction writes 1 KB without gaps.  (Lanes of 16 codes, whose two
+// stores leave gaps of 16 bytes between lanes, took 62 us where this takes 25: 8 x 8 heads of up to 4096 MXFP8 rows of 128,
+// 36 MB read and 134 MB written; ordinary stores instead of streaming ones 30 us.)
 template <int D, int FMT, bool F16>
 __global__ __launch_bounds__(256) void kv_gather_kernel(GatherParams p) {
-  constexpr int kE = FMT == MASE_KV_16BIT ? 8 : 16;
-  constexpr int kPieces = D / kE;
-  constexpr int kBytes = FMT == MASE_KV_16BIT ? 16 : (FMT == MASE_KV_MXFP4 ? 8 : 16);  // in storage
+  constexpr int kPieces = D / 8;
+  constexpr int kBytes = FMT == MASE_KV_16BIT ? 16 : (FMT == MASE_KV_MXFP4 ? 4 : 8);  // in storage
   const int b = blockIdx.z, h = blockIdx.y;
-  const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
-  const int slot = (int)(idx / kPieces), piece = (int)(idx % kPieces);
+  const int piece = (int)threadIdx.x % kPieces, slot = (int)blockIdx.x * (256 / kPieces) + (int)threadIdx.x / kPieces;
   if (slot >= p.max_length) return;
   const int length = kv_length(p.lengths[b], p.max_length, p.c.table_pages, p.c.page_shift);
-  uint32_t kw[kE / 2], vw[kE / 2];
-#pragma unroll
-  for (int j = 0; j < kE / 2; ++j) kw[j] = vw[j] = 0;
   const int page = slot < length ? kv_page(p.c.table + (size_t)b * p.c.table_stride, p.c.table_pages, p.c.page_shift, p.c.num_pages, slot) : -1;
+  uint32_t kw[4] = {0, 0, 0, 0}, vw[4] = {0, 0, 0, 0};
   if (page >= 0) {
     const int row = slot & ((1 << p.c.page_shift) - 1);
     uint32_t kc[kBytes / 4], vc[kBytes / 4];
@@ -225,24 +223,21 @@ __global__ __launch_bounds__(256) void kv_gather_kernel(GatherParams p) {
     kv_load<kBytes>(p.c.v + (size_t)page * p.c.v_page + (size_t)h * p.c.v_head + (size_t)row * p.c.v_slot + piece * kBytes, vc);
     float ks = 0.0f, vs = 0.0f;
     if constexpr (FMT != MASE_KV_16BIT) {
-      ks = kv_scale<FMT>(p.c.ks[key_scale_at<D>(p.c, page, h, row) + piece / 2]);
-      vs = kv_scale<FMT>(p.c.vs[value_scale_at<D>(p.c, page, h, row) + ((size_t)(piece / 2) << p.c.page_shift)]);
+      ks = kv_scale<FMT>(p.c.ks[key_scale_at<D>(p.c, page, h, row) + piece / 4]);
+      vs = kv_scale<FMT>(p.c.vs[value_scale_at<D>(p.c, page, h, row) + ((size_t)(piece / 4) << p.c.page_shift)]);
     }
-    kv_widen<FMT, F16, kE>(kc, ks, kw);
-    kv_widen<FMT, F16, kE>(vc, vs, vw);
+    kv_widen<FMT, F16, 8>(kc, ks, kw);
+    kv_widen<FMT, F16, 8>(vc, vs, vw);
   }
-  const size_t at = ((((size_t)b * p.c.heads + h) * p.max_length + slot) * D + piece * kE) * 2;
-#pragma unroll
-  for (int j = 0; j < kE / 8; ++j) {
-    store_nt((uint4*)(p.key + at) + j, make_uint4(kw[4 * j], kw[4 * j + 1], kw[4 * j + 2], kw[4 * j + 3]));
-    store_nt((uint4*)(p.value + at) + j, make_uint4(vw[4 * j], vw[4 * j + 1], vw[4 * j + 2], vw[4 * j + 3]));
-  }
+  const size_t at = ((((size_t)b * p.c.heads + h) * p.max_length + slot) * D + piece * 8) * 2;
+  store_nt((uint4*)(p.key + at), make_uint4(kw[0], kw[1], kw[2], kw[3]));
+  store_nt((uint4*)(p.value + at), make_uint4(vw[0], vw[1], vw[2], vw[3]));
 }
 
 template <int D, int FMT>
 void launch_gather(const GatherParams& p, int dtype, size_t batch, hipStream_t st) {
-  constexpr int kPieces = D / (FMT == MASE_KV_16BIT ? 8 : 16);
-  const dim3 grid(blocks_for((size_t)p.max_length * kPieces, 256), (unsigned)p.c.heads, (unsigned)batch), block(256);
+  constexpr int kPieces = D / 8;
+  const dim3 grid(blocks_for((size_t)p.max_length, 256 / kPieces), (unsigned)p.c.heads, (unsigned)batch), block(256);
   if (FMT == MASE_KV_16BIT || dtype == MASE_DT_BF16)
     hipLaunchKernelGGL((kv_gather_kernel<D, FMT, false>), grid, block, 0, st, p);
   else
@@ -280,14 +275,40 @@ __device__ __forceinline__ int lanes_below(uint64_t mask) {
   return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
 }
 
-// One work-group per (sequence, cached head).  The key of the keep-th largest slot by three histogram passes over 11, 11
-// and 10 bits of the keys; then the kept slots in slot order, by counts per wavefront (a wavefront owns a contiguous run
-// of slots) and ballots within it.  Weights and positions are read once per pass, from L2 after the first.
+// The bin of a histogram of keys, from the top, that the `want`-th largest key falls into, and how many keys lie in bins
+// above it.  All threads call it; hist has 2048 counts.
+__device__ __forceinline__ void find_bin(const uint32_t* hist, int want, int* sums, int* found, int tid, int lane, int wave) {
+  const int hi = (int)hist[2047 - 2 * tid], lo = (int)hist[2046 - 2 * tid];
+  int run = hi + lo;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(run, d, 64);
+    if (lane >= d) run += o;
+  }
+  if (lane == 63) sums[wave] = run;
+  __syncthreads();
+  int before = run - hi - lo;
+  for (int i = 0; i < wave; ++i) before += sums[i];
+  if (before < want && want <= before + hi + lo) {  // one thread
+    const bool upper = want <= before + hi;
+    found[0] = 2047 - 2 * tid - (upper ? 0 : 1);
+    found[1] = before + (upper ? 0 : hi);
+  }
+  __syncthreads();
+}
+
+// One work-group per (sequence, cached head); a wavefront owns a contiguous run of slots, 64 at a time, so that ranks in
+// slot order come from counts per wavefront and ballots within it.  The key of the keep-th largest slot is found by three
+// histograms over 11, 11 and 10 bits of the keys.  KPT > 0: rows of up to 1024 KPT slots, whose keys stay in registers;
+// KPT == 0: longer rows, whose keys are made anew from L2 for each pass.  What bounds it is the latency of its few dependent
+// steps, so weights and positions are read in runs of independent loads.
+template <int KPT>
 __global__ __launch_bounds__(kSelThreads) void kv_evict_select_kernel(EvictParams p) {
   __shared__ uint32_t hist[2048];
-  __shared__ int sums[kSelWaves], sums2[kSelWaves];
-  __shared__ int sel_bin, sel_above;
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ int sums[kSelWaves], sums2[kSelWaves], found[2];
+  constexpr int kRun = KPT == 32 || KPT == 64 ? 16 : 8;  // loads in flight
+  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const size_t rowi = (size_t)b * p.c.heads + h;
   const float* w = p.weights + rowi * p.capacity;
   const int32_t* pos = p.positions + rowi * p.capacity;
@@ -307,18 +328,66 @@ __global__ __launch_bounds__(kSelThreads) void kv_evict_select_kernel(EvictParam
     if (tid == 0) p.moves[rowi] = 0;
     return;
   }
+  const int turns = (n + kSelThreads - 1) / kSelThreads;  // of 64 slots, for each wavefront; at most KPT if that is not 0
+  const int s_lo = wave * turns * 64 + lane;               // this lane's first slot, the next ones 64 apart
   // the largest position
   int newest = -0x7FFFFFFF - 1;
-  for (int s = tid; s < n; s += kSelThreads) newest = max(newest, pos[s]);
+  for (int k = 0; k < turns; k += kRun) {
+    int v[kRun];
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) v[j] = pos[min(s_lo + 64 * (k + j), n - 1)];
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) newest = max(newest, v[j]);
+  }
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) newest = max(newest, __shfl_xor(newest, d, 64));
   if (lane == 0) sums[wave] = newest;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kSelWaves; ++i) newest = max(newest, sums[i]);
+  __syncthreads();
 
-  uint32_t prefix = 0, prefix_mask = 0;
-  int want = p.keep;  // how many of the slots that match the prefix are kept
+  // keys of kRun turns from k on (anything for slots that are not there)
+  auto there = [&](int k) __attribute__((always_inline)) { return k < turns && s_lo + 64 * k < n; };
+  auto make_keys = [&](int k, uint32_t* key) __attribute__((always_inline)) {
+    float wv[kRun];
+    int pv[kRun];
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) {
+      const int s = min(s_lo + 64 * (k + j), n - 1);
+      wv[j] = w[s];
+      pv[j] = pos[s];
+    }
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) key[j] = evict_key(wv[j], pv[j], newest, p);
+  };
+  uint32_t keys[KPT ? KPT : 1];
+  uint32_t cut = 0;      // the keep-th largest key
+  int want = p.keep;     // how many of the slots with that key are kept: the first ones
+  int gt = 0, eq = 0;    // this wavefront's slots above and at the cut
+  if constexpr (KPT > 0) {
+    static_assert(KPT % kRun == 0, "whole runs");
+#pragma unroll
+    for (int k = 0; k < KPT; k += kRun) {
+      if (k < turns) make_keys(k, keys + k);
+    }
+  }
+  // calls f(k, key) for each of this wavefront's turns of 64 slots
+  auto for_keys = [&](auto f) __attribute__((always_inline)) {
+    if constexpr (KPT > 0) {
+#pragma unroll
+      for (int k = 0; k < KPT; ++k)
+        if (k < turns) f(k, keys[k]);
+    } else {
+      for (int k = 0; k < turns; k += kRun) {
+        uint32_t key[kRun];
+        make_keys(k, key);
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) f(k + j, key[j]);
+      }
+    }
+  };
+  uint32_t cut_mask = 0;
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
@@ -326,54 +395,29 @@ __global__ __launch_bounds__(kSelThreads) void kv_evict_select_kernel(EvictParam
     hist[tid] = 0;
     hist[tid + 1024] = 0;
     __syncthreads();
-    for (int s0 = wave * 64; s0 < n; s0 += kSelThreads) {
-      const int s = s0 + lane;
-      const uint32_t key = s < n ? evict_key(w[s], pos[s], newest, p) : 0u;
-      const bool in = s < n && (key & prefix_mask) == prefix;
+    for_keys([&](int k, uint32_t key) __attribute__((always_inline)) {
+      const bool in = there(k) && (key & cut_mask) == cut;
       const uint32_t bin = (key >> shift) & (bins - 1);
       // equal keys are common (tokens never attended to): those of the first lane's bin are added at once
       const uint64_t act = __builtin_amdgcn_ballot_w64(in);
       if (act != 0) {
-        const uint32_t lead = (uint32_t)__shfl((int)bin, (int)__builtin_ctzll(act), 64);
+        const uint32_t lead = (uint32_t)__builtin_amdgcn_readlane((int)bin, (int)__builtin_ctzll(act));
         const uint64_t same = __builtin_amdgcn_ballot_w64(in && bin == lead);
         if (in && bin != lead) atomicAdd(&hist[bin], 1u);
         if (lane == 0) atomicAdd(&hist[lead], (uint32_t)__popcll(same));
       }
-    }
+    });
     __syncthreads();
-    // counts of the bins from the top: thread t has bins 2047 - 2t and 2046 - 2t
-    const int hi = (int)hist[2047 - 2 * tid], lo = (int)hist[2046 - 2 * tid];
-    int run = hi + lo;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(run, d, 64);
-      if (lane >= d) run += o;
-    }
-    if (lane == 63) sums[wave] = run;
-    __syncthreads();
-    int before = run - hi - lo;
-    for (int i = 0; i < wave; ++i) before += sums[i];
-    if (before < want && want <= before + hi + lo) {  // one thread: the kept ones end in one of its bins
-      const bool upper = want <= before + hi;
-      sel_bin = 2047 - 2 * tid - (upper ? 0 : 1);
-      sel_above = before + (upper ? 0 : hi);
-    }
-    __syncthreads();
-    want -= sel_above;
-    prefix |= (uint32_t)sel_bin << shift;
-    prefix_mask |= (bins - 1) << shift;
+    find_bin(hist, want, sums, found, tid, lane, wave);
+    want -= found[1];
+    cut |= (uint32_t)found[0] << shift;
+    cut_mask |= (bins - 1) << shift;
     __syncthreads();
   }
-  // keys above `prefix` are kept, and the first `want` that equal it
-  const int run_len = ((n + kSelThreads - 1) / kSelThreads) * 64;
-  const int s_lo = wave * run_len, s_hi = min(n, s_lo + run_len);
-  int gt = 0, eq = 0;
-  for (int s0 = s_lo; s0 < s_hi; s0 += 64) {
-    const int s = s0 + lane;
-    const uint32_t key = s < s_hi ? evict_key(w[s], pos[s], newest, p) : 0u;
-    gt += __popcll(__builtin_amdgcn_ballot_w64(s < s_hi && key > prefix));
-    eq += __popcll(__builtin_amdgcn_ballot_w64(s < s_hi && key == prefix));
-  }
+  for_keys([&](int k, uint32_t key) __attribute__((always_inline)) {
+    gt += __popcll(__builtin_amdgcn_ballot_w64(there(k) && key > cut));
+    eq += __popcll(__builtin_amdgcn_ballot_w64(there(k) && key == cut));
+  });
   if (lane == 0) {
     sums[wave] = gt;
     sums2[wave] = eq;
@@ -387,16 +431,13 @@ __global__ __launch_bounds__(kSelThreads) void kv_evict_select_kernel(EvictParam
   }
   int32_t* holes = p.holes + rowi * p.keep;
   int32_t* fillers = p.fillers + rowi * p.keep;
-  for (int s0 = s_lo; s0 < s_hi; s0 += 64) {
-    const int s = s0 + lane;
-    const bool in = s < s_hi;
-    const float wv = in ? w[s] : 0.0f;
-    const int pv = in ? pos[s] : 0;
-    const uint32_t key = evict_key(wv, pv, newest, p);
-    const uint64_t gm = __builtin_amdgcn_ballot_w64(in && key > prefix), em = __builtin_amdgcn_ballot_w64(in && key == prefix);
+  auto emit = [&](int k, uint32_t key, float wv, int pv) __attribute__((always_inline)) {
+    const int s = s_lo + 64 * k;
+    const bool in = there(k), above = in && key > cut, at = in && key == cut;
+    const uint64_t gm = __builtin_amdgcn_ballot_w64(above), em = __builtin_amdgcn_ballot_w64(at);
     const int eq_before = eq + lanes_below(em);
     const int kept_before = gt + lanes_below(gm) + min(eq_before, want);
-    const bool kept = in && (key > prefix || (key == prefix && eq_before < want));
+    const bool kept = above || (at && eq_before < want);
     if (in && s < p.keep) {
       if (kept) {
         wo[s] = wv;
@@ -410,6 +451,29 @@ __global__ __launch_bounds__(kSelThreads) void kv_evict_select_kernel(EvictParam
     if (in && s == p.keep) p.moves[rowi] = p.keep - kept_before;
     gt += __popcll(gm);
     eq += __popcll(em);
+  };
+  auto emit_run = [&](int k, const uint32_t* key) __attribute__((always_inline)) {
+    float wv[kRun];
+    int pv[kRun];
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) {
+      const int s = min(s_lo + 64 * (k + j), n - 1);
+      wv[j] = w[s];
+      pv[j] = pos[s];
+    }
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) emit(k + j, key[j], wv[j], pv[j]);
+  };
+  if constexpr (KPT > 0) {
+#pragma unroll
+    for (int k = 0; k < KPT; k += kRun)
+      if (k < turns) emit_run(k, keys + k);
+  } else {
+    for (int k = 0; k < turns; k += kRun) {
+      uint32_t key[kRun];
+      make_keys(k, key);
+      emit_run(k, key);
+    }
   }
 }
 
@@ -592,8 +656,12 @@ extern "C" int mase_paged_kv_evict(const mase_paged_kv* cache, const int32_t* le
   p.recent = (int)recent;
   p.first = (int)first;
   hipStream_t st = (hipStream_t)stream;
-  hipLaunchKernelGGL(kv_evict_select_kernel, dim3((unsigned)cache->kv_heads, (unsigned)cache->batch), dim3(kSelThreads), 0,
-                     st, p);
+  const dim3 grid((unsigned)cache->kv_heads, (unsigned)cache->batch);
+  const size_t most = max_length < capacity ? max_length : capacity;  // slots of a row
+  if (most <= 8 * kSelThreads) hipLaunchKernelGGL((kv_evict_select_kernel<8>), grid, dim3(kSelThreads), 0, st, p);
+  else if (most <= 32 * kSelThreads) hipLaunchKernelGGL((kv_evict_select_kernel<32>), grid, dim3(kSelThreads), 0, st, p);
+  else if (most <= 64 * kSelThreads) hipLaunchKernelGGL((kv_evict_select_kernel<64>), grid, dim3(kSelThreads), 0, st, p);
+  else hipLaunchKernelGGL((kv_evict_select_kernel<0>), grid, dim3(kSelThreads), 0, st, p);
   if (max_length > keep && capacity > keep) MASE_KV_DISPATCH(cache, launch_evict_move, p, cache->batch, st);
   return hipGetLastError() == hipSuccess ? MASE_OK : MASE_ERR_LAUNCH;
 }

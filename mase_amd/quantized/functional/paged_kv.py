@@ -26,6 +26,7 @@ its slots being absent.  Inference only: no gradient is recorded.
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -37,6 +38,7 @@ from ..._tables import log2_table
 KV_FORMATS = tuple(_lib.KV_FORMATS)
 _HEAD_DIMS = (64, 128, 256)
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
 def _int32(t: Tensor, name: str, shape, device) -> int:
@@ -92,37 +94,43 @@ def _pool(what: str, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, kv_fo
                         _lib.DTYPE_CODE[dtype])
 
 
+_entry = {}  # entry points of the library by name
+
+
 def _call(name: str, device: torch.device, *args) -> None:
     """one entry point on the device's current stream, with that device current"""
-    fn = getattr(_lib.load(), name)
-    if torch.cuda.current_device() == device.index:
-        rc = fn(*args, _raw_stream(device.index))
+    fn = _entry.get(name)
+    if fn is None:
+        fn = _entry[name] = getattr(_lib.load(), name)
+    index = device.index
+    if _current_device() == index:
+        rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, _raw_stream(device.index))
+            rc = fn(*args, _raw_stream(index))
     if rc:
         _lib.check(rc, name)
 
 
-def _bytes(name: str, device: torch.device, *args) -> int:
-    fn = getattr(_lib.load(), name)
-    if torch.cuda.current_device() == device.index:
-        return fn(*args)
-    with torch.cuda.device(device):
-        return fn(*args)
+@lru_cache(maxsize=4096)
+def _workspace_bytes(name: str, index: int, *sizes: int) -> int:
+    """what an entry point needs for these sizes on this device (it depends on nothing else)"""
+    with torch.cuda.device(index):
+        return getattr(_lib.load(), name)(*sizes)
 
 
 def _states(t: Tensor) -> Tensor:
     """a tensor whose rows are contiguous and 16-byte aligned; a copy where the given one's are not"""
-    st = t.stride()
-    if st[-1] != 1 or t.data_ptr() % 16 or any(s % 8 for s, n in zip(st[:-1], t.shape) if n > 1):
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:  # rows are multiples of 64 elements
+        return t
+    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % 8 for s in _strides(t)):
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
 def _strides(t: Tensor) -> Tuple[int, ...]:
     """element strides of all but the last dimension, those of dimensions of size one (which mean nothing) as zero"""
-    return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape))
+    return tuple([s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape)])
 
 
 def _own_rows(t: Tensor, dtype: torch.dtype, batch: int, heads: int, least: int, device) -> bool:
@@ -251,8 +259,8 @@ def paged_attention_decode(query: Tensor, k_pages: Tensor, v_pages: Tensor, page
     out = torch.empty((batch, heads, head_dim), dtype=query.dtype, device=device)
     if batch == 0:
         return out
-    n = _bytes("mase_paged_attention_decode_workspace_bytes", device, batch, heads, kv_heads, head_dim, c.format, max_length,
-               wp is not None)
+    n = _workspace_bytes("mase_paged_attention_decode_workspace_bytes", device.index, batch, heads, kv_heads, head_dim, c.format,
+                         max_length, int(wp is not None))
     ws = torch.empty(n, dtype=torch.uint8, device=device)
     _call("mase_paged_attention_decode", device, ctypes.addressof(c), query.data_ptr(), *_strides(query), heads, lp, max_length,
           float(scaling), mp, mcode, m_b, wp, w_b, w_h, out.data_ptr(), ws.data_ptr(), n)
@@ -287,7 +295,7 @@ def paged_kv_evict(k_pages: Tensor, v_pages: Tensor, page_table: Tensor, lengths
     lp = _int32(lengths, "lengths", (c.batch,), device)
     new_weights, new_positions, new_lengths = torch.empty_like(weights), torch.empty_like(positions), torch.empty_like(lengths)
     if c.batch:
-        n = _bytes("mase_paged_kv_evict_workspace_bytes", device, c.batch, c.kv_heads, keep)
+        n = _workspace_bytes("mase_paged_kv_evict_workspace_bytes", device.index, c.batch, c.kv_heads, keep)
         ws = torch.empty(n, dtype=torch.uint8, device=device)
         _call("mase_paged_kv_evict", device, ctypes.addressof(c), lp, max_length, weights.data_ptr(), pp, capacity, keep, recent,
               first, new_weights.data_ptr(), new_positions.data_ptr(), new_lengths.data_ptr(), ws.data_ptr(), n)
