@@ -481,16 +481,18 @@ __device__ __forceinline__ void ml_add(float& top, float& sum, float4& acc, floa
 
 constexpr int kWeightSlots = 1024;  // per work-group
 
-// Joins the pieces of cut rows.  grid (x, row, sequence): a work-group takes `items` (a power of two from 16 to 256) of the
-// row's rows * D / 4 groups of four outputs, 256 / items threads sharing the pieces of each; the host takes as few items as
-// make 256 work-groups of all rows.  The pieces' sums are added in a fixed order.
+// Joins the pieces of cut rows (blocks x < joins) and, with weights, adds the probabilities to them (the blocks behind).
+// grid (x, row, sequence).
+//
+// Joining: a work-group takes `items` (a power of two from 16 to 256) of the row's rows * D / 4 groups of four outputs,
+// 256 / items threads sharing the pieces of each; the host takes as few items as make 256 work-groups of all rows.  The
+// pieces' sums are added in a fixed order.
 template <int D, bool F16>
-__global__ __launch_bounds__(256) void paged_decode_join_kernel(DecodeParams p, int items) {
-  __shared__ __attribute__((aligned(16))) float4 acc_s[256];
-  __shared__ float top_s[256], sum_s[256];
-  const int rh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
-  const int row_heads = p.c.heads * p.head_tiles;
-  const Pieces q = row_pieces(p, b, rh, row_heads);
+__device__ __forceinline__ void join_pieces(const DecodeParams& p, int items, int rh, int b, float* lds) {
+  float4* acc_s = (float4*)lds;  // [256], then [256] reference points and [256] sums
+  float *top_s = lds + 1024, *sum_s = lds + 1280;
+  const int tid = threadIdx.x;
+  const Pieces q = row_pieces(p, b, rh, p.c.heads * p.head_tiles);
   if (q.count == 1) return;
   const int hk = rh / p.head_tiles, tile = rh % p.head_tiles;
   const int rows = min(kHeadTile, p.group - tile * kHeadTile);
@@ -520,18 +522,16 @@ __global__ __launch_bounds__(256) void paged_decode_join_kernel(DecodeParams p, 
   *(uint2*)(p.out + (bh * D + col) * 2) = y;
 }
 
-// Adds the probabilities of kWeightSlots slots, summed over the query heads of a cached head, to the weights.
-// grid (share of the slots, cached head, sequence).
-__global__ __launch_bounds__(256) void paged_decode_weights_kernel(DecodeParams p) {
-  __shared__ float top_s[kMaxGroup], inv_s[kMaxGroup];
-  const int hk = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int row_heads = p.c.heads * p.head_tiles;
+// Weights: the probabilities of kWeightSlots slots, summed over the query heads of a cached head.
+__device__ __forceinline__ void add_weights(const DecodeParams& p, int share, int hk, int b, float* lds) {
+  float *top_s = lds, *inv_s = lds + kMaxGroup;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const size_t bh0 = (size_t)b * p.heads + (size_t)hk * p.group;
-  const int s0 = (int)blockIdx.x * kWeightSlots;
+  const int s0 = share * kWeightSlots;
   const int length = kv_length(p.lengths[b], p.max_length, p.c.table_pages, p.c.page_shift);
   if (s0 >= length) return;
   for (int h = wave; h < p.group; h += 4) {
-    const Pieces q = row_pieces(p, b, hk * p.head_tiles + h / kHeadTile, row_heads);
+    const Pieces q = row_pieces(p, b, hk * p.head_tiles + h / kHeadTile, p.c.heads * p.head_tiles);
     float top = -__builtin_inff(), sum = 0.0f;
     float4 none = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     const float4 zero = none;
@@ -567,6 +567,14 @@ __global__ __launch_bounds__(256) void paged_decode_weights_kernel(DecodeParams 
     const int s = s0 + 256 * j + tid;
     if (s < length) wrow[s] += acc[j];
   }
+}
+
+template <int D, bool F16>
+__global__ __launch_bounds__(256) void paged_decode_join_kernel(DecodeParams p, int joins, int items) {
+  __shared__ __attribute__((aligned(16))) float lds[1536];
+  const int rh = blockIdx.y, b = blockIdx.z;
+  if ((int)blockIdx.x < joins) join_pieces<D, F16>(p, items, rh, b, lds);
+  else if (rh % p.head_tiles == 0) add_weights(p, (int)blockIdx.x - joins, rh / p.head_tiles, b, lds);
 }
 
 // What a call launches and keeps between its two kernels.
@@ -615,14 +623,13 @@ int launch_decode(const DecodeParams& p, const DecodePlan& d, hipStream_t st) {
   const void* fn = (const void*)paged_decode_kernel<D, FMT, F16, EXTRA>;
   if (!set_dynamic_lds_once(attr_done, fn, (int)(kMost > kOnly ? kMost : kOnly))) return MASE_ERR_LAUNCH;
   hipLaunchKernelGGL((paged_decode_kernel<D, FMT, F16, EXTRA>), dim3((unsigned)d.groups), dim3(256), lds, st, p);
-  if (d.join) {
-    const size_t rows = (size_t)p.c.heads * d.head_tiles, all = (size_t)d.tile_rows * (D / 4);
-    int items = 256;
-    while (items > 16 && ((size_t)items / 2 >= all || (size_t)p.batch * rows * ((all + items - 1) / items) < 256)) items /= 2;
-    hipLaunchKernelGGL((paged_decode_join_kernel<D, F16>), dim3(blocks_for(all, (size_t)items), (unsigned)rows, (unsigned)p.batch), dim3(256), 0, st, p, items);
-  }
-  if (EXTRA != kPlain && p.scores != nullptr && p.max_length > 0)
-    hipLaunchKernelGGL(paged_decode_weights_kernel, dim3(blocks_for((size_t)p.max_length, kWeightSlots), (unsigned)p.c.heads, (unsigned)p.batch), dim3(256), 0, st, p);
+  const size_t rows = (size_t)p.c.heads * d.head_tiles, all = (size_t)d.tile_rows * (D / 4);
+  int items = 256;
+  while (items > 16 && ((size_t)items / 2 >= all || (size_t)p.batch * rows * ((all + items - 1) / items) < 256)) items /= 2;
+  const unsigned joins = d.join ? blocks_for(all, (size_t)items) : 0;
+  const unsigned shares = EXTRA != kPlain && p.scores != nullptr ? blocks_for((size_t)p.max_length, kWeightSlots) : 0;
+  if (joins + shares > 0)
+    hipLaunchKernelGGL((paged_decode_join_kernel<D, F16>), dim3(joins + shares, (unsigned)rows, (unsigned)p.batch), dim3(256), 0, st, p, (int)joins, items);
   return MASE_OK;
 }
 

@@ -261,7 +261,6 @@ struct EvictParams {
   int max_length, capacity, keep, recent, first;
 };
 
-constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64;
 
 // a number that orders slots: protected ones above every weight, NaN below
 __device__ __forceinline__ uint32_t evict_key(float w, int pos, int newest, const EvictParams& p) {
@@ -275,38 +274,69 @@ __device__ __forceinline__ int lanes_below(uint64_t mask) {
   return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
 }
 
-// The bin of a histogram of keys, from the top, that the `want`-th largest key falls into, and how many keys lie in bins
-// above it.  All threads call it; hist has 2048 counts.
-__device__ __forceinline__ void find_bin(const uint32_t* hist, int want, int* sums, int* found, int tid, int lane, int wave) {
-  const int hi = (int)hist[2047 - 2 * tid], lo = (int)hist[2046 - 2 * tid];
-  int run = hi + lo;
+// sum of a value over this lane and those below it (quad and row shifts, then the last lanes of the rows before)
+__device__ __forceinline__ int scan64(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+
+// sum of the first `wave` of a work-group's per-wavefront numbers
+template <int WAVES>
+__device__ __forceinline__ int sum_before(const int* sums, int wave) {
+  int s = 0;
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int o = __shfl_up(run, d, 64);
-    if (lane >= d) run += o;
+  for (int i = 0; i < WAVES - 1; ++i) s += i < wave ? sums[i] : 0;
+  return s;
+}
+
+// Histogram of 256 bins in kCopies interleaved copies: the lanes of a wavefront that meet in a bin (tokens never attended
+// to, weights of one binade) are spread over as many addresses in as many banks.
+constexpr int kCopies = 8;
+
+// The bin, from the top, that the `want`-th largest key falls into (found[0]), and how many keys lie in bins above it
+// (found[1]); the histogram is zero afterwards.  All threads (at least 256) call it.
+__device__ __forceinline__ void find_bin(uint32_t* hist, int want, int* sums, int* found, int tid, int lane, int wave) {
+  int mine = 0, run = 0;
+  const int bin = 255 - tid;
+  if (wave < 4) {
+    uint4* c = (uint4*)(hist + bin * kCopies);
+    const uint4 u = c[0], v = c[1];
+    c[0] = c[1] = make_uint4(0, 0, 0, 0);
+    mine = (int)(u.x + u.y + u.z + u.w + v.x + v.y + v.z + v.w);
+    run = scan64(mine);
+    if (lane == 63) sums[wave] = run;
   }
-  if (lane == 63) sums[wave] = run;
   __syncthreads();
-  int before = run - hi - lo;
-  for (int i = 0; i < wave; ++i) before += sums[i];
-  if (before < want && want <= before + hi + lo) {  // one thread
-    const bool upper = want <= before + hi;
-    found[0] = 2047 - 2 * tid - (upper ? 0 : 1);
-    found[1] = before + (upper ? 0 : hi);
+  if (wave < 4) {
+    const int before = run - mine + sum_before<4>(sums, wave);
+    if (before < want && want <= before + mine) {  // one thread
+      found[0] = bin;
+      found[1] = before;
+    }
   }
   __syncthreads();
 }
 
 // One work-group per (sequence, cached head); a wavefront owns a contiguous run of slots, 64 at a time, so that ranks in
-// slot order come from counts per wavefront and ballots within it.  The key of the keep-th largest slot is found by three
-// histograms over 11, 11 and 10 bits of the keys.  KPT > 0: rows of up to 1024 KPT slots, whose keys stay in registers;
-// KPT == 0: longer rows, whose keys are made anew from L2 for each pass.  What bounds it is the latency of its few dependent
-// steps, so weights and positions are read in runs of independent loads.
-template <int KPT>
-__global__ __launch_bounds__(kSelThreads) void kv_evict_select_kernel(EvictParams p) {
-  __shared__ uint32_t hist[2048];
-  __shared__ int sums[kSelWaves], sums2[kSelWaves], found[2];
-  constexpr int kRun = KPT == 32 || KPT == 64 ? 16 : 8;  // loads in flight
+// slot order come from counts per wavefront and ballots within it.  The key of the keep-th largest slot is found by four
+// histograms over 8 bits of the keys each.  HELD: the row's keys stay in LDS (rows of up to kHeldSlots); otherwise
+// they are made anew from L2 for each pass.
+// It is bound by the latency of its dependent steps on one CU (two reads of the row, four histograms, the ranks): 43 us for
+// 64 rows of 20001 .. 32768 slots, 11 us for 8 rows of 2047.  Weights and positions are read in runs of independent loads (one at a time, each waiting for L2: 103 us);
+// keys in registers with every turn unrolled were no faster (45 us: the code itself came from memory).
+constexpr int kHeldSlots = 36864;
+
+template <int WAVES, bool HELD>
+__global__ __launch_bounds__(64 * WAVES) void kv_evict_select_kernel(EvictParams p) {
+  constexpr int kThreads = 64 * WAVES, kRun = 8;  // turns whose loads are in flight together
+  extern __shared__ uint32_t held[];              // HELD: [turns * kThreads] keys by slot
+  __shared__ __attribute__((aligned(16))) uint32_t hist[256 * kCopies];
+  __shared__ int sums[WAVES], sums2[WAVES], found[2];
   const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const size_t rowi = (size_t)b * p.c.heads + h;
@@ -316,165 +346,161 @@ __global__ __launch_bounds__(kSelThreads) void kv_evict_select_kernel(EvictParam
   int32_t* po = p.positions_out + rowi * p.capacity;
   const int n = kv_length(p.lengths[b], min(p.max_length, p.capacity), p.c.table_pages, p.c.page_shift);
   if (h == 0 && tid == 0) p.lengths_out[b] = min(n, p.keep);
-  for (int s = min(n, p.keep) + tid; s < p.capacity; s += kSelThreads) {
-    wo[s] = 0.0f;
-    po[s] = -1;
-  }
   if (n <= p.keep) {
-    for (int s = tid; s < n; s += kSelThreads) {
-      wo[s] = w[s];
-      po[s] = pos[s];
+    for (int s = tid; s < p.capacity; s += kThreads) {
+      wo[s] = s < n ? w[s] : 0.0f;
+      po[s] = s < n ? pos[s] : -1;
     }
     if (tid == 0) p.moves[rowi] = 0;
     return;
   }
-  const int turns = (n + kSelThreads - 1) / kSelThreads;  // of 64 slots, for each wavefront; at most KPT if that is not 0
-  const int s_lo = wave * turns * 64 + lane;               // this lane's first slot, the next ones 64 apart
-  // the largest position
+  const int turns = (n + kThreads - 1) / kThreads;    // of 64 slots, for each wavefront
+  const int s_lo = wave * turns * 64 + lane;          // this lane's first slot, the next ones 64 apart
+  auto there = [&](int k) __attribute__((always_inline)) { return k < turns && s_lo + 64 * k < n; };
+
+  // the largest position; HELD: keys but for the recent slots' protection, which needs it
   int newest = -0x7FFFFFFF - 1;
   for (int k = 0; k < turns; k += kRun) {
-    int v[kRun];
+    int pv[kRun];
+    float wv[kRun];
 #pragma unroll
-    for (int j = 0; j < kRun; ++j) v[j] = pos[min(s_lo + 64 * (k + j), n - 1)];
+    for (int j = 0; j < kRun; ++j) {
+      const int s = min(s_lo + 64 * (k + j), n - 1);
+      pv[j] = pos[s];
+      wv[j] = HELD ? w[s] : 0.0f;
+    }
 #pragma unroll
-    for (int j = 0; j < kRun; ++j) newest = max(newest, v[j]);
+    for (int j = 0; j < kRun; ++j) {
+      newest = max(newest, pv[j]);
+      if (HELD && k + j < turns) held[s_lo + 64 * (k + j)] = evict_key(wv[j], pv[j], 0x7FFFFFFF, p);
+    }
   }
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) newest = max(newest, __shfl_xor(newest, d, 64));
   if (lane == 0) sums[wave] = newest;
+  for (int i = tid; i < 256 * kCopies; i += kThreads) hist[i] = 0;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kSelWaves; ++i) newest = max(newest, sums[i]);
-  __syncthreads();
-
-  // keys of kRun turns from k on (anything for slots that are not there)
-  auto there = [&](int k) __attribute__((always_inline)) { return k < turns && s_lo + 64 * k < n; };
-  auto make_keys = [&](int k, uint32_t* key) __attribute__((always_inline)) {
-    float wv[kRun];
-    int pv[kRun];
+  for (int i = 0; i < WAVES; ++i) newest = max(newest, sums[i]);
+  if (HELD && p.recent > 0) {
+    for (int k = 0; k < turns; k += kRun) {
+      int pv[kRun];
 #pragma unroll
-    for (int j = 0; j < kRun; ++j) {
-      const int s = min(s_lo + 64 * (k + j), n - 1);
-      wv[j] = w[s];
-      pv[j] = pos[s];
-    }
+      for (int j = 0; j < kRun; ++j) pv[j] = pos[min(s_lo + 64 * (k + j), n - 1)];
 #pragma unroll
-    for (int j = 0; j < kRun; ++j) key[j] = evict_key(wv[j], pv[j], newest, p);
-  };
-  uint32_t keys[KPT ? KPT : 1];
-  uint32_t cut = 0;      // the keep-th largest key
-  int want = p.keep;     // how many of the slots with that key are kept: the first ones
-  int gt = 0, eq = 0;    // this wavefront's slots above and at the cut
-  if constexpr (KPT > 0) {
-    static_assert(KPT % kRun == 0, "whole runs");
-#pragma unroll
-    for (int k = 0; k < KPT; k += kRun) {
-      if (k < turns) make_keys(k, keys + k);
+      for (int j = 0; j < kRun; ++j)
+        if (k + j < turns && (long long)pv[j] > (long long)newest - p.recent) held[s_lo + 64 * (k + j)] = 0xFFFFFFFFu;
     }
   }
   // calls f(k, key) for each of this wavefront's turns of 64 slots
   auto for_keys = [&](auto f) __attribute__((always_inline)) {
-    if constexpr (KPT > 0) {
-#pragma unroll
-      for (int k = 0; k < KPT; ++k)
-        if (k < turns) f(k, keys[k]);
-    } else {
+    if constexpr (HELD) {
       for (int k = 0; k < turns; k += kRun) {
         uint32_t key[kRun];
-        make_keys(k, key);
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) key[j] = held[s_lo + 64 * min(k + j, turns - 1)];
 #pragma unroll
         for (int j = 0; j < kRun; ++j) f(k + j, key[j]);
       }
+    } else {
+      for (int k = 0; k < turns; k += kRun) {
+        float wv[kRun];
+        int pv[kRun];
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) {
+          const int s = min(s_lo + 64 * (k + j), n - 1);
+          wv[j] = w[s];
+          pv[j] = pos[s];
+        }
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) f(k + j, evict_key(wv[j], pv[j], newest, p));
+      }
     }
   };
-  uint32_t cut_mask = 0;
+  uint32_t cut = 0, cut_mask = 0;  // the keep-th largest key, as far as it is known
+  int want = p.keep;               // how many of the slots with that key are kept: the first ones
 #pragma unroll 1
-  for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
-    const uint32_t bins = pass == 2 ? 1024u : 2048u;
-    hist[tid] = 0;
-    hist[tid + 1024] = 0;
-    __syncthreads();
+  for (int shift = 24; shift >= 0; shift -= 8) {
     for_keys([&](int k, uint32_t key) __attribute__((always_inline)) {
-      const bool in = there(k) && (key & cut_mask) == cut;
-      const uint32_t bin = (key >> shift) & (bins - 1);
-      // equal keys are common (tokens never attended to): those of the first lane's bin are added at once
-      const uint64_t act = __builtin_amdgcn_ballot_w64(in);
-      if (act != 0) {
-        const uint32_t lead = (uint32_t)__builtin_amdgcn_readlane((int)bin, (int)__builtin_ctzll(act));
-        const uint64_t same = __builtin_amdgcn_ballot_w64(in && bin == lead);
-        if (in && bin != lead) atomicAdd(&hist[bin], 1u);
-        if (lane == 0) atomicAdd(&hist[lead], (uint32_t)__popcll(same));
-      }
+      if (there(k) && (key & cut_mask) == cut) atomicAdd(&hist[((key >> shift) & 255u) * kCopies + (lane & (kCopies - 1))], 1u);
     });
     __syncthreads();
     find_bin(hist, want, sums, found, tid, lane, wave);
     want -= found[1];
     cut |= (uint32_t)found[0] << shift;
-    cut_mask |= (bins - 1) << shift;
-    __syncthreads();
+    cut_mask |= 255u << shift;
   }
+  int gt = 0, eq = 0;  // slots above and at the cut: the lane's, the wavefront's, then those before the slot in hand
   for_keys([&](int k, uint32_t key) __attribute__((always_inline)) {
-    gt += __popcll(__builtin_amdgcn_ballot_w64(there(k) && key > cut));
-    eq += __popcll(__builtin_amdgcn_ballot_w64(there(k) && key == cut));
+    gt += there(k) && key > cut ? 1 : 0;
+    eq += there(k) && key == cut ? 1 : 0;
   });
+  gt = __builtin_amdgcn_readlane(scan64(gt), 63);
+  eq = __builtin_amdgcn_readlane(scan64(eq), 63);
   if (lane == 0) {
     sums[wave] = gt;
     sums2[wave] = eq;
   }
   __syncthreads();
-  gt = 0;
-  eq = 0;
-  for (int i = 0; i < wave; ++i) {
-    gt += sums[i];
-    eq += sums2[i];
-  }
+  gt = sum_before<WAVES>(sums, wave);
+  eq = sum_before<WAVES>(sums2, wave);
   int32_t* holes = p.holes + rowi * p.keep;
   int32_t* fillers = p.fillers + rowi * p.keep;
-  auto emit = [&](int k, uint32_t key, float wv, int pv) __attribute__((always_inline)) {
-    const int s = s_lo + 64 * k;
-    const bool in = there(k), above = in && key > cut, at = in && key == cut;
-    const uint64_t gm = __builtin_amdgcn_ballot_w64(above), em = __builtin_amdgcn_ballot_w64(at);
-    const int eq_before = eq + lanes_below(em);
-    const int kept_before = gt + lanes_below(gm) + min(eq_before, want);
-    const bool kept = above || (at && eq_before < want);
-    if (in && s < p.keep) {
-      if (kept) {
-        wo[s] = wv;
-        po[s] = pv;
-      } else {
-        holes[s - kept_before] = s;
-      }
-    } else if (kept) {
-      fillers[kept_before] = s;  // kept_before < keep: exactly keep slots are kept
-    }
-    if (in && s == p.keep) p.moves[rowi] = p.keep - kept_before;
-    gt += __popcll(gm);
-    eq += __popcll(em);
-  };
-  auto emit_run = [&](int k, const uint32_t* key) __attribute__((always_inline)) {
+#pragma unroll 1
+  for (int k = 0; k < turns; k += kRun) {
     float wv[kRun];
     int pv[kRun];
+    uint32_t kv[kRun];
 #pragma unroll
     for (int j = 0; j < kRun; ++j) {
       const int s = min(s_lo + 64 * (k + j), n - 1);
       wv[j] = w[s];
       pv[j] = pos[s];
+      if (HELD) kv[j] = held[s_lo + 64 * min(k + j, turns - 1)];
     }
 #pragma unroll
-    for (int j = 0; j < kRun; ++j) emit(k + j, key[j], wv[j], pv[j]);
-  };
-  if constexpr (KPT > 0) {
-#pragma unroll
-    for (int k = 0; k < KPT; k += kRun)
-      if (k < turns) emit_run(k, keys + k);
-  } else {
-    for (int k = 0; k < turns; k += kRun) {
-      uint32_t key[kRun];
-      make_keys(k, key);
-      emit_run(k, key);
+    for (int j = 0; j < kRun; ++j) {
+      const int s = s_lo + 64 * (k + j);
+      const bool in = there(k + j);
+      const uint32_t key = HELD ? kv[j] : evict_key(wv[j], pv[j], newest, p);
+      const bool above = in && key > cut, at = in && key == cut;
+      const uint64_t gm = __builtin_amdgcn_ballot_w64(above), em = __builtin_amdgcn_ballot_w64(at);
+      const int eq_before = eq + lanes_below(em);
+      const int kept_before = gt + lanes_below(gm) + min(eq_before, want);
+      const bool kept = above || (at && eq_before < want);
+      if (in) {
+        if (s < p.keep) {
+          if (kept) {
+            wo[s] = wv[j];
+            po[s] = pv[j];
+          } else {
+            holes[s - kept_before] = s;
+          }
+        } else if (kept) {
+          fillers[kept_before] = s;  // kept_before < keep: exactly keep slots are kept
+        }
+        if (s == p.keep) p.moves[rowi] = p.keep - kept_before;
+      }
+      gt += __popcll(gm);
+      eq += __popcll(em);
     }
   }
+  for (int s = p.keep + tid; s < p.capacity; s += kThreads) {
+    wo[s] = 0.0f;
+    po[s] = -1;
+  }
+}
+
+template <int WAVES, bool HELD>
+int launch_evict_select(const EvictParams& p, size_t batch, size_t most, hipStream_t st) {
+  // keys by slot, in whole turns of the work-group
+  const size_t lds = HELD ? (most + 64 * WAVES - 1) / (64 * WAVES) * (64 * WAVES) * sizeof(uint32_t) : 0;
+  if (HELD && WAVES == 16) {
+    static std::atomic<uint64_t> attr_done{0};
+    if (!set_dynamic_lds_once(attr_done, (const void*)kv_evict_select_kernel<WAVES, HELD>, kHeldSlots * (int)sizeof(uint32_t))) return MASE_ERR_LAUNCH;
+  }
+  hipLaunchKernelGGL((kv_evict_select_kernel<WAVES, HELD>), dim3((unsigned)p.c.heads, (unsigned)batch), dim3(64 * WAVES), lds, st, p);
+  return MASE_OK;
 }
 
 // Moves kept rows from behind `keep` into the free slots: sources and targets are disjoint, so the order does not matter.
@@ -656,12 +682,12 @@ extern "C" int mase_paged_kv_evict(const mase_paged_kv* cache, const int32_t* le
   p.recent = (int)recent;
   p.first = (int)first;
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((unsigned)cache->kv_heads, (unsigned)cache->batch);
   const size_t most = max_length < capacity ? max_length : capacity;  // slots of a row
-  if (most <= 8 * kSelThreads) hipLaunchKernelGGL((kv_evict_select_kernel<8>), grid, dim3(kSelThreads), 0, st, p);
-  else if (most <= 32 * kSelThreads) hipLaunchKernelGGL((kv_evict_select_kernel<32>), grid, dim3(kSelThreads), 0, st, p);
-  else if (most <= 64 * kSelThreads) hipLaunchKernelGGL((kv_evict_select_kernel<64>), grid, dim3(kSelThreads), 0, st, p);
-  else hipLaunchKernelGGL((kv_evict_select_kernel<0>), grid, dim3(kSelThreads), 0, st, p);
+  // short rows: fewer wavefronts, whose barriers are shorter
+  const int src = most <= 4096 ? launch_evict_select<4, true>(p, cache->batch, most, st)
+                  : most <= (size_t)kHeldSlots ? launch_evict_select<16, true>(p, cache->batch, most, st)
+                                               : launch_evict_select<16, false>(p, cache->batch, most, st);
+  if (src != MASE_OK) return src;
   if (max_length > keep && capacity > keep) MASE_KV_DISPATCH(cache, launch_evict_move, p, cache->batch, st);
   return hipGetLastError() == hipSuccess ? MASE_OK : MASE_ERR_LAUNCH;
 }
