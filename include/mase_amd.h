@@ -469,10 +469,10 @@ int mase_paged_kv_gather(const mase_paged_kv* cache, const int32_t* lengths, siz
 /* Attention of one new token per sequence over its cached slots: x = scaling * (q . k) + mask, p = softmax(x),
  * out = sum p v for q, out [batch][heads][head_dim] of `dtype` (q by element strides of batch and head, multiples of 8,
  * rows 16-byte aligned; out contiguous); query head h reads cached head h / (heads / kv_heads).  Scores, softmax statistics
- * and sums are fp32; probabilities are rounded to `dtype` for the product with the values.
+ * and sums are fp32; probabilities enter the product with the values as two numbers of `dtype`, the rounded one and the rest.
  * mask (optional): added to the scores of all heads, [batch][max_length] of mask_dtype (the cache's dtype or fp32) with an
  * element stride of batch (0: one row for all); a slot whose mask is -inf is left out whatever its keys and values hold.
- * A row without a slot gives zeros.
+ * A row without a slot gives zeros.  An infinite value in a slot that counts gives NaN.
  * weights (optional, fp32) [batch][kv_heads][...] by element strides of batch and head: entry t grows by the probabilities
  * of slot t summed over the query heads of its cached head, in a fixed order.
  * The cache is split over its length; the parts (and with weights the scores) pass through `workspace`,

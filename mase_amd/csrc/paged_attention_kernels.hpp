@@ -319,8 +319,11 @@ __global__ __launch_bounds__(256, (Rows<D, FMT>::kPerCu)) void paged_decode_kern
       }
       const float ms = m == -__builtin_inff() ? 0.0f : m;
       {
-        // fp16 probabilities are held 2^kShift up, where small ones keep their bits (fp16 loses them below 2^-14)
-        uint32_t pf[4];
+        // Probabilities enter the product with the values as two 16-bit numbers, the rounded one and what it left out (about 16
+        // bits of bf16, 22 of fp16): rounded once, they alone would be as far off as the rounded result.  The second product
+        // costs matrix instructions that the loads leave free.  fp16 ones are held 2^kShift up, where small ones keep their
+        // bits (fp16 loses them below 2^-14).
+        uint32_t pf[4], pl[4];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           float ex[4];
@@ -329,8 +332,12 @@ __global__ __launch_bounds__(256, (Rows<D, FMT>::kPerCu)) void paged_decode_kern
             ex[r] = __builtin_amdgcn_exp2f((x[t][r] - ms) * kLog2e + kShift);
             l += ex[r];
           }
-          pf[2 * t] = kv_pack2<F16>(ex[0], ex[1]);
-          pf[2 * t + 1] = kv_pack2<F16>(ex[2], ex[3]);
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const uint32_t w = kv_pack2<F16>(ex[2 * r], ex[2 * r + 1]);
+            pf[2 * t + r] = w;
+            pl[2 * t + r] = kv_pack2<F16>(ex[2 * r] - half_of<F16>(w, 0), ex[2 * r + 1] - half_of<F16>(w, 1));
+          }
         }
         float vscale[8];
         if constexpr (R::kPacked) {
@@ -369,6 +376,8 @@ __global__ __launch_bounds__(256, (Rows<D, FMT>::kPerCu)) void paged_decode_kern
           }
           o[2 * np] = mfma16<F16>(f0, pf, o[2 * np]);
           o[2 * np + 1] = mfma16<F16>(f1, pf, o[2 * np + 1]);
+          o[2 * np] = mfma16<F16>(f0, pl, o[2 * np]);
+          o[2 * np + 1] = mfma16<F16>(f1, pl, o[2 * np + 1]);
           if (R::kPacked && (np & 1)) __builtin_amdgcn_sched_barrier(0);
         }
       }

@@ -119,28 +119,6 @@ def attend(q, k, v, scaling, mask, dtype):
     keep = torch.ones(n, dtype=torch.bool) if mask is None else mask > -math.inf
     if not bool(keep.any()):
         return out, probs, tol_o, tol_p
-    for h in range(heads):
-        kk, vv = k[h // (heads // kvh)][keep], v[h // (heads // kvh)][keep]
-        add = 0.0 if mask is None else mask[keep].double()
-        prod = q[h].double() * kk
-        x = prod.sum(-1) * scaling + add
-        e = torch.exp(x - x.max())
-        p = e / e.sum()
-        out[h], probs[h, keep] = p @ vv, p
-        # fp32: a dot product of dim exact products is off by at most dim half-steps of the sum of magnitudes (any order),
-        # scaling and mask round once each; the exponent (x - m) log2e rounds twice and the exponential once or so; the
-        # sum of n positive terms and the division add (n / 128 + 16) half-steps (n / 128 terms a lane, then trees)
-        half = HALF[torch.float32]
-        dx = (dim + 2) * half * float(prod.abs().sum(-1).max()) * abs(scaling) + 2 * half * float(x[x > -1e30].abs().max()) if bool((x > -1e30).any()) else 0.0
-        span = float((x.max() - x).clamp(max=120).max())
-        rel = 2 * (dx + 4 * half * span) + (n / 128 + 24) * half
-        tol_p[h, keep] = p * rel + 2.0 ** -120
-        # probabilities round to dtype before the product with the values (fp16 ones are held 2^11 up and lose bits below
-        # 2^-14 there: at most 2^-25 2^-11 each), the result rounds once more, the sums over n run in fp32
-        mass = p @ vv.abs()
-        tiny = n * 2.0 ** -36 * vv.abs().amax(0) if dtype == torch.float16 else 0.0
-        tol_o[h] = HALF[dtype] * out[h].abs() + mass * (HALF[dtype] * (1 + HALF[dtype]) + rel + (n / 32 + 24) * half) + tiny + 2.0 ** -24
-    return out, probs, tol_o, tol_p
 
 
 def evict(pos, w, n, keep, recent, first):
@@ -148,6 +126,7 @@ def evict(pos, w, n, keep, recent, first):
     if n <= keep:
         return list(range(n))
     newest = max(pos[:n])
+
     def rank(s):  # protected ones, then by weight, NaN last, ties to the lowest slot
         if pos[s] < first or pos[s] > newest - recent:
             return (0, 0.0, s)
