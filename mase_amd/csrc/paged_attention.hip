@@ -18,7 +18,7 @@ extern "C" size_t mase_paged_attention_decode_workspace_bytes(size_t batch, size
                                                               int format, size_t max_length, int with_weights) {
   using namespace mase;
   if (batch == 0 || batch > 65535 || kv_heads == 0 || heads == 0 || heads % kv_heads != 0 || heads / kv_heads > (size_t)kMaxGroup ||
-      max_length > 0x7FFFFF00u || (head_dim != 64 && head_dim != 128 && head_dim != 256))
+      max_length > 0x7FFF0000u || (head_dim != 64 && head_dim != 128 && head_dim != 256))
     return 0;
   size_t need = 0;
   DecodeCall c{};
@@ -42,7 +42,7 @@ extern "C" int mase_paged_attention_decode(const mase_paged_kv* cache, const voi
   const int rc = paged_kv_params(cache, p.c);
   if (rc != MASE_OK) return rc;
   if (heads == 0 || heads % cache->kv_heads != 0 || heads / cache->kv_heads > (size_t)kMaxGroup) return MASE_ERR_SHAPE;
-  if (max_length > 0x7FFFFF00u) return MASE_ERR_SHAPE;
+  if (max_length > 0x7FFF0000u) return MASE_ERR_SHAPE;  // a step looks a little past the last slot
   if (!(scaling > -3.0e38f && scaling < 3.0e38f)) return MASE_ERR_PARAM;
   if (mask != nullptr && mask_dtype != cache->dtype && mask_dtype != MASE_DT_F32) return MASE_ERR_DTYPE;
   if (cache->batch == 0) return MASE_OK;

@@ -653,7 +653,7 @@ int decode_call(DecodeCall& c) {
   if (!aligned16(c.workspace)) return MASE_ERR_ALIGN;
   // units are counted in 32 bits: all of them, rounded up to whole shares, and a share with a row's on top
   const size_t row = c.max_length / Rows<D, FMT>::kUnit + 1;
-  if (row * c.batch > 0x3FFFFFFFu || d.groups > 0x7FFFFFFFu) return MASE_ERR_SHAPE;
+  if (row * c.batch > 0x3FFFFFFFu || c.kv_heads * d.head_tiles > 65535u) return MASE_ERR_SHAPE;
   c.p.plan = (uint32_t*)c.workspace;
   float* f = (float*)(c.workspace + d.plan_bytes);
   c.p.part_o = f;

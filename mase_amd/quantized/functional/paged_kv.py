@@ -288,6 +288,8 @@ def paged_kv_evict(k_pages: Tensor, v_pages: Tensor, page_table: Tensor, lengths
         raise ValueError(f"{what}: keep must be at least 1 and hold first + recent tokens, got keep={keep}, recent={recent}, first={first}")
     if max_length < 0 or max_length > c.table_pages * c.page_size:
         raise ValueError(f"{what}: max_length must be between 0 and the table's {c.table_pages * c.page_size} slots, got {max_length}")
+    if keep >= max_length:  # no sequence is longer: nothing moves, and no room for moves is needed
+        keep, recent, first = max(max_length, 1), 0, 0
     capacity = weights.shape[-1] if weights.dim() == 3 else 0
     shape = (c.batch, c.kv_heads, capacity)
     if weights.dtype != torch.float32 or tuple(weights.shape) != shape or capacity < max(max_length, 1) or weights.device != device or not weights.is_contiguous():

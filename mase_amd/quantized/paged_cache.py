@@ -58,6 +58,7 @@ class PagedKVCache:
             self._ks = torch.zeros((*shape, head_dim // 32), dtype=torch.uint8, device=self.device)
             self._vs = torch.zeros((*shape[:3], head_dim // 32, page_size), dtype=torch.uint8, device=self.device)
         self._table = torch.full((batch_size, table_pages), -1, dtype=torch.int32, device=self.device)
+        self.device = self._table.device  # with its index, whichever device is current later
         self._free = list(range(self.num_pages - 1, -1, -1))
         self._pages: List[List[int]] = [[] for _ in range(batch_size)]
         # per layer: slots held and tokens seen, on the host and on the device

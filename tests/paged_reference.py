@@ -119,6 +119,35 @@ def attend(q, k, v, scaling, mask, dtype):
     keep = torch.ones(n, dtype=torch.bool) if mask is None else mask > -math.inf
     if not bool(keep.any()):
         return out, probs, tol_o, tol_p
+    half = HALF[torch.float32]
+    for h in range(heads):
+        kk, vv = k[h // (heads // kvh)][keep], v[h // (heads // kvh)][keep]
+        add = 0.0 if mask is None else mask[keep].double()
+        prod = q[h].double() * kk
+        x = prod.sum(-1) * scaling + add
+        e = torch.exp(x - x.max())
+        p = e / e.sum()
+        out[h], probs[h, keep] = p @ vv, p
+        # fp32: a dot product of dim exact products is off by at most dim half-steps of the sum of magnitudes (any order),
+        # scaling and mask round once each; the exponent (x - m) log2e rounds twice and the exponential once or so; the
+        # sum of n positive terms and the division add (n / 128 + 16) half-steps (n / 128 terms a lane, then trees)
+        dx = (dim + 2) * half * float(prod.abs().sum(-1).max()) * abs(scaling)
+        if bool((x > -1e30).any()):
+            dx += 2 * half * float(x[x > -1e30].abs().max())
+        if dtype == torch.float16:  # a code's value below 2^-14 is widened to within half a step of 2^-24
+            dx += abs(scaling) * float(q[h].double().abs().sum()) * 2.0 ** -25
+        span = float((x.max() - x).clamp(max=120).max())
+        rel = 2 * (dx + 4 * half * span) + (n / 128 + 24) * half
+        tol_p[h, keep] = p * rel + 2.0 ** -120
+        # a probability enters the product with the values as a number of dtype and the rest as another: what is left out is
+        # at most HALF of the rest, which is at most HALF of it (fp16: held 2^11 up, bits below 2^-24 there are lost, half a
+        # step of 2^-25 2^-11 each); the result rounds to dtype (fp16 below 2^-14: half a step is 2^-25, once for the result
+        # and at most once, the probabilities adding up to 1, for code values widened to fp16); the sums over 2 n products
+        # run in fp32
+        mass = p @ vv.abs()
+        tiny = n * 2.0 ** -36 * vv.abs().amax(0) + 2.0 ** -24 if dtype == torch.float16 else 2.0 ** -126
+        tol_o[h] = HALF[dtype] * out[h].abs() + mass * (HALF[dtype] ** 2 + rel + (n / 16 + 24) * half) * (1 + HALF[dtype]) + tiny
+    return out, probs, tol_o, tol_p
 
 
 def evict(pos, w, n, keep, recent, first):

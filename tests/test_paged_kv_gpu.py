@@ -230,6 +230,26 @@ def test_decode_page_sizes(dev, page):
     check_decode(dev, p, 4, 9, weights=True)
 
 
+def test_decode_many_short_sequences(dev):
+    """more sequences than a work-group has threads, more than the launch has shares; some empty"""
+    g = gen(65)
+    n = 700
+    k, v = (torch.randn(n, 1, 16, 64, generator=g).bfloat16() for _ in range(2))
+    table = torch.randperm(n, generator=g).to(torch.int32).view(n, 1)
+    lengths = torch.randint(0, 17, (n,), generator=g).to(torch.int32)
+    q = torch.randn(n, 4, 64, generator=g).bfloat16()
+    w = torch.zeros(n, 1, 16, device=dev)
+    out = F().paged_attention_decode(q.to(dev), k.to(dev), v.to(dev), table.to(dev), lengths.to(dev), 16, weights=w).cpu().double()
+    rows = torch.arange(16) < lengths[:, None]
+    kk, vv = k[table[:, 0].long(), 0].double(), v[table[:, 0].long(), 0].double()
+    x = torch.where(rows[:, None], q.double() @ kk.transpose(1, 2) / 8, -math.inf)
+    p = torch.where(lengths[:, None, None] > 0, torch.softmax(x, -1), 0.0)
+    want = p @ vv
+    # fp32 statistics (1e-5 covers them at 16 slots and scores below 10) and one rounding
+    assert bool(((out - want).abs() <= HALF[torch.bfloat16] * want.abs() + 1e-5 * (p @ vv.abs()) + 1e-30).all())
+    assert bool(((w[:, 0].cpu().double() - p.sum(1)).abs() <= 1e-5 * 4).all()) and not bool(out[lengths == 0].any())
+
+
 @pytest.mark.parametrize("fmt", [None, "mxfp4"])
 def test_decode_splits_one_long_sequence_and_joins(dev, fmt):
     p = Pool(gen(10), [40001], 1, 128, 256, fmt, torch.bfloat16)
@@ -463,6 +483,17 @@ def test_evict_orders_odd_weights(dev):
     check_evict(dev, p, w, pos, 90, 3, 1)
     w[1] = math.nan
     check_evict(dev, p, w, pos, 101, 0, 0)
+
+
+def test_evict_to_more_than_there_is_copies_what_there_is(dev):
+    p = Pool(gen(63), [30, 64], 2, 64, 16, None, torch.bfloat16)
+    cap = p.table.shape[1] * 16
+    w, pos = torch.rand(2, 2, cap, generator=gen(64)), torch.arange(cap, dtype=torch.int32).expand(2, 2, cap).contiguous()
+    for keep, recent in ((64, 64), (1 << 30, 1 << 29)):  # the second would take 32 GB to list moves that cannot be
+        kw, nw, npos, nlen = _run_evict(dev, p, w, pos, keep, recent, 5 if keep > 64 else 0)
+        assert nlen.tolist() == [30, 64] and torch.equal(nw[1], w[1]) and torch.equal(npos[0, :, :30], pos[0, :, :30])
+        assert not bool(nw[0, :, 30:].any()) and bool((npos[0, :, 30:] == -1).all())
+        assert_bits_equal(kw["k_pages"], p.k)
 
 
 @pytest.mark.parametrize("n,keep", [(5000, 4096), (70001, 35000), (33000, 100)])

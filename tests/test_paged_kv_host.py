@@ -128,6 +128,8 @@ def test_entry_points_refuse_bad_arguments(lib):
 
     assert decode(q=None) == -1 and decode(lengths=None) == -1 and decode(out=None) == -1
     assert decode(heads=3) == -2 and decode(heads=0) == -2 and decode(heads=2 * 257) == -2 and decode(n=1 << 40) == -2
+    many, _p, _b3 = _pool(kv_heads=8192)  # 9 tiles of 16 query heads for each: too many rows for a grid
+    assert lib.mase_paged_attention_decode(ctypes.addressof(many), p, 128, 64, 8192 * 144, p, 16, 0.1, None, 0, 0, None, 0, 0, p, p, 1 << 40, None) == -2
     assert decode(scaling=float("nan")) == -5 and decode(scaling=float("inf")) == -5
     assert decode(mask=p, mdt=2) == -4 and decode(q=p + 8) == -3 and decode(qs=(128, 60)) == -3 and decode(out=p + 8) == -3
     assert decode(w=p, ws=None, wsb=0) == -7 and decode(w=p, wsb=16) == -7 and decode(w=p, ws=p + 8) == -3
