@@ -157,7 +157,8 @@ __global__ __launch_bounds__(256, (Rows<D, FMT>::kPerCu)) void paged_decode_kern
 #pragma unroll 1
   for (bool first_piece = true;; first_piece = false) {
     const int e = min(n_units, a + left);  // this row's units a .. e - 1
-    const int lo = a * R::kUnit, hi = min(e * R::kUnit, length);
+    // (a lane's value read back keeps what follows from it, the addresses of pages above all, in scalar registers)
+    const int lo = a * R::kUnit, hi = __builtin_amdgcn_readfirstlane(min(e * R::kUnit, length));
     const scalar_int* table = (const scalar_int*)(p.c.table + (size_t)b * p.c.table_stride);
 
     uint32_t qf[D / 32][4];
@@ -185,6 +186,12 @@ __global__ __launch_bounds__(256, (Rows<D, FMT>::kPerCu)) void paged_decode_kern
     constexpr int kMaskSize = EXTRA == kMaskF32 ? 4 : 2, kMaskWords = kMaskSize;  // bytes of a value, words of four
     uint32_t mk[2][kMaskWords];
     const unsigned char* mask_row = kMask ? p.mask + (size_t)b * p.mask_sb * kMaskSize : nullptr;
+    // lane offsets from a tile's first row
+    const uint32_t k_lane = (uint32_t)i * p.c.k_slot + (uint32_t)(g * R::kKeyBytes);
+    uint32_t v_lane[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v_lane[j] = (uint32_t)(4 * g + j) * p.c.v_slot + (uint32_t)(i * R::kValBytes);
+    const uint32_t vs_lane = ((uint32_t)((i * R::kC) / 32) << p.c.page_shift) + (uint32_t)(4 * g);
     auto load_keys = [&](const int* page, const int* row) __attribute__((always_inline)) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -192,9 +199,9 @@ __global__ __launch_bounds__(256, (Rows<D, FMT>::kPerCu)) void paged_decode_kern
         const unsigned char* base = p.c.k + (size_t)pg * p.c.k_page + (size_t)hk * p.c.k_head + (size_t)row[t] * p.c.k_slot;
 #pragma unroll
         for (int u = 0; u < R::kKeyLoads; ++u)
-          kv_load<R::kKeyBytes>(base + (uint32_t)i * p.c.k_slot + (uint32_t)((u * 4 + g) * R::kKeyBytes), kr[t][u]);
+          kv_load<R::kKeyBytes>(base + (k_lane + (uint32_t)(u * 4 * R::kKeyBytes)), kr[t][u]);
         if constexpr (R::kPacked)
-          kv_load<D / 32>((const unsigned char*)p.c.ks + ((((size_t)pg * p.c.heads + hk) << p.c.page_shift) + row[t]) * (D / 32) + i * (D / 32), ksc[t]);
+          kv_load<D / 32>((const unsigned char*)p.c.ks + ((((size_t)pg * p.c.heads + hk) << p.c.page_shift) + row[t]) * (D / 32) + (uint32_t)(i * (D / 32)), ksc[t]);
       }
     };
     auto load_values = [&](const int* page, const int* row) __attribute__((always_inline)) {
@@ -204,9 +211,9 @@ __global__ __launch_bounds__(256, (Rows<D, FMT>::kPerCu)) void paged_decode_kern
         const unsigned char* base = p.c.v + (size_t)pg * p.c.v_page + (size_t)hk * p.c.v_head + (size_t)row[t] * p.c.v_slot;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          kv_load<R::kValBytes>(base + (uint32_t)(4 * g + j) * p.c.v_slot + (uint32_t)(i * R::kValBytes), vr[4 * t + j]);
+          kv_load<R::kValBytes>(base + v_lane[j], vr[4 * t + j]);
         if constexpr (R::kPacked)
-          vsc[t] = *(const uint32_t*)(p.c.vs + (((((size_t)pg * p.c.heads + hk) * (D / 32)) + (i * R::kC) / 32) << p.c.page_shift) + row[t] + 4 * g);
+          vsc[t] = *(const uint32_t*)(p.c.vs + ((((size_t)pg * p.c.heads + hk) * (D / 32)) << p.c.page_shift) + row[t] + vs_lane);
       }
     };
     // what is added to the scores of slots s0 + 16 t + 4 g + r, as it lies in memory, four at a time (rows have any
