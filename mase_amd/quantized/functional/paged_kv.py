@@ -25,7 +25,7 @@ its slots being absent.  Inference only: no gradient is recorded.
 """
 from __future__ import annotations
 
-import ctypes
+import struct
 from functools import lru_cache
 from typing import Optional, Tuple
 
@@ -37,61 +37,85 @@ from ..._tables import log2_table
 
 KV_FORMATS = tuple(_lib.KV_FORMATS)
 _HEAD_DIMS = (64, 128, 256)
+_STATE_CODES = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
 
 
 def _int32(t: Tensor, name: str, shape, device) -> int:
-    if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or t.device != device or not t.is_contiguous():
+    if t.dtype != torch.int32 or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)} on {device}, got {t.dtype} "
                          f"{tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _pool(what: str, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, kv_format, k_scales, v_scales, dtype) -> _lib.PagedKv:
-    """the pool as the C ABI takes it, after the checks that the host can make"""
-    if kv_format not in _lib.KV_FORMATS:
-        raise ValueError(f"{what}: kv_format must be one of {KV_FORMATS}, got {kv_format!r}")
-    device = k_pages.device
-    _lib.require_device(k_pages, what)
-    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
-        raise ValueError(f"{what}: k_pages and v_pages must be [pages, kv_heads, page_size, head_dim] alike, got "
-                         f"{tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
-    pages, heads, page_size, width = k_pages.shape
-    head_dim = 2 * width if kv_format == "mxfp4" else width
-    if head_dim not in _HEAD_DIMS:
-        raise ValueError(f"{what}: head_dim must be one of {_HEAD_DIMS}, got {head_dim}")
-    if page_size < 16 or page_size > 4096 or page_size & (page_size - 1):
-        raise ValueError(f"{what}: page_size must be a power of two from 16 to 4096, got {page_size}")
-    if dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"{what}: states must be bfloat16 or float16, got {dtype}")
-    want = dtype if kv_format is None else (torch.int8 if kv_format == "mxint8" else torch.uint8)
-    if k_pages.dtype != want or v_pages.dtype != want:
-        raise ValueError(f"{what}: pages must be {want} for kv_format={kv_format!r} and {dtype} states, got {k_pages.dtype} "
-                         f"and {v_pages.dtype}")
-    item = k_pages.element_size()
-    ks, vs = (*_strides(k_pages), k_pages.stride(3)), (*_strides(v_pages), v_pages.stride(3))
-    if v_pages.device != device or ks[3] != 1 or vs[3] != 1:
-        raise ValueError(f"{what}: k_pages and v_pages must be on one device with contiguous rows")
-    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.device != device or (
-            page_table.shape[1] > 1 and page_table.stride(1) != 1) or (
-            page_table.shape[0] > 1 and page_table.stride(0) < page_table.shape[1]):
-        raise ValueError(f"{what}: page_table must be an int32 tensor [batch, table_pages] on {device} with contiguous rows of its own for each sequence")
-    sk = sv = None
-    if kv_format is not None:
-        if k_scales is None or v_scales is None:
-            raise ValueError(f"{what}: kv_format={kv_format!r} needs k_scales and v_scales")
-        shapes = ((pages, heads, page_size, head_dim // 32), (pages, heads, head_dim // 32, page_size))
-        for name, t, shape in (("k_scales", k_scales, shapes[0]), ("v_scales", v_scales, shapes[1])):
-            if t.dtype != torch.uint8 or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
-                raise ValueError(f"{what}: {name} must be a contiguous uint8 tensor {shape} on {device}, got {t.dtype} "
-                                 f"{tuple(t.shape)} on {t.device}")
-        sk, sv = k_scales.data_ptr(), v_scales.data_ptr()
-    batch, table_pages = page_table.shape
-    return _lib.PagedKv(k_pages.data_ptr(), v_pages.data_ptr(), sk, sv, page_table.data_ptr(), pages, page_size, heads,
-                        head_dim, batch, table_pages, max(page_table.stride(0), table_pages), ks[0] * item, ks[1] * item,
-                        ks[2] * item, vs[0] * item, vs[1] * item, vs[2] * item, _lib.KV_FORMATS[kv_format],
-                        _lib.DTYPE_CODE[dtype])
+# mase_paged_kv of the C ABI as one packed record (the layout of _lib.PagedKv, which a test compares)
+_record = struct.Struct("@5P13N2i").pack
+
+
+class _Pool:
+    """a pool after the checks that the host can make: its record for the C ABI and the sizes that the callers look at"""
+
+    __slots__ = ("record", "device", "batch", "kv_heads", "head_dim", "slots", "format")
+
+    def __init__(self, what: str, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, kv_format, k_scales, v_scales, dtype):
+        code = _lib.KV_FORMATS.get(kv_format)
+        if code is None:
+            raise ValueError(f"{what}: kv_format must be one of {KV_FORMATS}, got {kv_format!r}")
+        if not k_pages.is_cuda:
+            _lib.require_device(k_pages, what)
+        device = self.device = k_pages.device
+        shape = k_pages.shape
+        if len(shape) != 4 or v_pages.shape != shape:
+            raise ValueError(f"{what}: k_pages and v_pages must be [pages, kv_heads, page_size, head_dim] alike, got "
+                             f"{tuple(shape)} and {tuple(v_pages.shape)}")
+        pages, heads, page_size, width = shape
+        head_dim = 2 * width if code == 4 else width
+        if head_dim not in _HEAD_DIMS:
+            raise ValueError(f"{what}: head_dim must be one of {_HEAD_DIMS}, got {head_dim}")
+        if page_size < 16 or page_size > 4096 or page_size & (page_size - 1):
+            raise ValueError(f"{what}: page_size must be a power of two from 16 to 4096, got {page_size}")
+        dtype_code = _STATE_CODES.get(dtype)
+        if dtype_code is None:
+            raise ValueError(f"{what}: states must be bfloat16 or float16, got {dtype}")
+        want = dtype if code == 0 else (torch.int8 if code == 1 else torch.uint8)
+        if k_pages.dtype != want or v_pages.dtype != want:
+            raise ValueError(f"{what}: pages must be {want} for kv_format={kv_format!r} and {dtype} states, got {k_pages.dtype} "
+                             f"and {v_pages.dtype}")
+        kp, kh, ks, k1 = k_pages.stride()
+        vp, vh, vs, v1 = v_pages.stride()
+        if v_pages.device != device or k1 != 1 or v1 != 1:
+            raise ValueError(f"{what}: k_pages and v_pages must be on one device with contiguous rows")
+        # strides of dimensions of size one mean nothing; a stride of zero would have pages or heads share their memory
+        if pages == 1:
+            kp = vp = 16
+        if heads == 1:
+            kh = vh = 16
+        if not (kp and kh and ks and vp and vh and vs):
+            raise ValueError(f"{what}: k_pages and v_pages must not be expanded tensors")
+        if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.device != device:
+            raise ValueError(f"{what}: page_table must be an int32 tensor [batch, table_pages] on {device}")
+        batch, table_pages = page_table.shape
+        tb, t1 = page_table.stride()
+        if batch <= 1:
+            tb = table_pages
+        if tb < table_pages or (t1 != 1 and table_pages > 1):
+            raise ValueError(f"{what}: page_table must have contiguous rows, each sequence its own")
+        sk = sv = 0
+        if code:
+            if k_scales is None or v_scales is None:
+                raise ValueError(f"{what}: kv_format={kv_format!r} needs k_scales and v_scales")
+            for name, t, want_shape in (("k_scales", k_scales, (pages, heads, page_size, head_dim // 32)),
+                                        ("v_scales", v_scales, (pages, heads, head_dim // 32, page_size))):
+                if t.dtype != torch.uint8 or t.shape != want_shape or t.device != device or not t.is_contiguous():
+                    raise ValueError(f"{what}: {name} must be a contiguous uint8 tensor {want_shape} on {device}, got {t.dtype} "
+                                     f"{tuple(t.shape)} on {t.device}")
+            sk, sv = k_scales.data_ptr(), v_scales.data_ptr()
+        item = 2 if code == 0 else 1
+        self.batch, self.kv_heads, self.head_dim, self.slots, self.format = batch, heads, head_dim, table_pages * page_size, code
+        self.record = _record(k_pages.data_ptr(), v_pages.data_ptr(), sk, sv, page_table.data_ptr(), pages, page_size, heads, head_dim,
+                              batch, table_pages, tb, kp * item, kh * item, ks * item, vp * item, vh * item, vs * item, code,
+                              dtype_code)
 
 
 _entry = {}  # entry points of the library by name
@@ -130,20 +154,22 @@ def _states(t: Tensor) -> Tensor:
 
 def _strides(t: Tensor) -> Tuple[int, ...]:
     """element strides of all but the last dimension, those of dimensions of size one (which mean nothing) as zero"""
-    return tuple([s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape)])
+    return tuple([s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)])[:-1]
 
 
 def _own_rows(t: Tensor, dtype: torch.dtype, batch: int, heads: int, least: int, device) -> bool:
     """whether t is ``[batch, heads, at least least]`` of dtype on device with contiguous rows that share no memory"""
-    if t.dtype != dtype or t.dim() != 3 or tuple(t.shape[:2]) != (batch, heads) or t.shape[2] < least or t.device != device:
+    if t.dtype != dtype or t.dim() != 3 or t.device != device:
+        return False
+    b, h, n = t.shape
+    if b != batch or h != heads or n < least:
         return False
     sb, sh, s1 = t.stride()
-    n = t.shape[2]
     return (n <= 1 or s1 == 1) and (heads == 1 or sh >= n) and (batch == 1 or sb >= (heads - 1) * (sh if heads > 1 else 0) + n)
 
 
 def _no_grad(what: str, *tensors: Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    if any([t.requires_grad for t in tensors]) and torch.is_grad_enabled():
         raise _lib.MaseAmdError(f"{what} is for inference and records no gradient: call it under torch.no_grad() or on detached tensors")
 
 
@@ -158,7 +184,7 @@ def paged_kv_append(key: Tensor, value: Tensor, k_pages: Tensor, v_pages: Tensor
     ``first_positions[b] + j`` (default ``starts[b] + j``).  Tokens without a slot in the table are not written."""
     what = "paged_kv_append"
     _no_grad(what, key, value)
-    c = _pool(what, k_pages, v_pages, page_table, kv_format, k_scales, v_scales, key.dtype)
+    c = _Pool(what, k_pages, v_pages, page_table, kv_format, k_scales, v_scales, key.dtype)
     device = k_pages.device
     if key.dim() != 4 or value.shape != key.shape or value.dtype != key.dtype or (key.shape[0], key.shape[1], key.shape[3]) != (c.batch, c.kv_heads, c.head_dim):
         raise ValueError(f"{what}: key and value must be [{c.batch}, {c.kv_heads}, tokens, {c.head_dim}] of one type, got "
@@ -174,7 +200,7 @@ def paged_kv_append(key: Tensor, value: Tensor, k_pages: Tensor, v_pages: Tensor
     pos_b = pos_h = 0
     if positions is not None:
         # an entry is written for every slot of the table that a token goes to
-        least = c.table_pages * c.page_size
+        least = c.slots
         if not _own_rows(positions, torch.int32, c.batch, c.kv_heads, least, device):
             raise ValueError(f"{what}: positions must be int32 [{c.batch}, {c.kv_heads}, at least {least}] on {device} with contiguous rows")
         pp, pos_b, pos_h = positions.data_ptr(), positions.stride(0), positions.stride(1)
@@ -184,7 +210,7 @@ def paged_kv_append(key: Tensor, value: Tensor, k_pages: Tensor, v_pages: Tensor
     tab = None
     if kv_format is not None:
         tab = log2_table(key.dtype if kv_format == "mxint8" else torch.float32, device).data_ptr()
-    _call("mase_paged_kv_append", device, ctypes.addressof(c), key.data_ptr(), value.data_ptr(), key.shape[2],
+    _call("mase_paged_kv_append", device, c.record, key.data_ptr(), value.data_ptr(), key.shape[2],
           *_strides(key), *_strides(value), sp, cp, pp, pos_b, pos_h, fp, tab)
 
 
@@ -198,7 +224,7 @@ def paged_kv_gather(k_pages: Tensor, v_pages: Tensor, page_table: Tensor, length
         if kv_format is not None:
             raise ValueError(f"{what}: dtype is needed with kv_format={kv_format!r}")
         dtype = k_pages.dtype
-    c = _pool(what, k_pages, v_pages, page_table, kv_format, k_scales, v_scales, dtype)
+    c = _Pool(what, k_pages, v_pages, page_table, kv_format, k_scales, v_scales, dtype)
     device = k_pages.device
     max_length = int(max_length)
     if max_length < 0:
@@ -206,7 +232,7 @@ def paged_kv_gather(k_pages: Tensor, v_pages: Tensor, page_table: Tensor, length
     out = torch.empty((2, c.batch, c.kv_heads, max_length, c.head_dim), dtype=dtype, device=device)
     key, value = out[0], out[1]
     if out.numel():
-        _call("mase_paged_kv_gather", device, ctypes.addressof(c), _int32(lengths, "lengths", (c.batch,), device), max_length,
+        _call("mase_paged_kv_gather", device, c.record, _int32(lengths, "lengths", (c.batch,), device), max_length,
               key.data_ptr(), value.data_ptr())
     return key, value
 
@@ -227,7 +253,7 @@ def paged_attention_decode(query: Tensor, k_pages: Tensor, v_pages: Tensor, page
     cached head.  ``max_length`` fixes how the work is split: one value for all calls of a captured step."""
     what = "paged_attention_decode"
     _no_grad(what, query)
-    c = _pool(what, k_pages, v_pages, page_table, kv_format, k_scales, v_scales, query.dtype)
+    c = _Pool(what, k_pages, v_pages, page_table, kv_format, k_scales, v_scales, query.dtype)
     device, batch, kv_heads, head_dim = k_pages.device, c.batch, c.kv_heads, c.head_dim
     if query.dim() != 3 or query.shape[0] != batch or query.shape[2] != head_dim or query.shape[1] % kv_heads or query.shape[1] == 0:
         raise ValueError(f"{what}: query must be [{batch}, a multiple of {kv_heads}, {head_dim}], got {tuple(query.shape)}")
@@ -237,8 +263,8 @@ def paged_attention_decode(query: Tensor, k_pages: Tensor, v_pages: Tensor, page
     if heads // kv_heads > 256:
         raise ValueError(f"{what}: at most 256 query heads for one cached head, got {heads // kv_heads}")
     max_length = int(max_length)
-    if max_length < 0 or max_length > c.table_pages * c.page_size:
-        raise ValueError(f"{what}: max_length must be between 0 and the table's {c.table_pages * c.page_size} slots, got {max_length}")
+    if max_length < 0 or max_length > c.slots:
+        raise ValueError(f"{what}: max_length must be between 0 and the table's {c.slots} slots, got {max_length}")
     if scaling is None:
         scaling = head_dim ** -0.5
     query = _states(query)
@@ -263,7 +289,7 @@ def paged_attention_decode(query: Tensor, k_pages: Tensor, v_pages: Tensor, page
     n = _workspace_bytes("mase_paged_attention_decode_workspace_bytes", device.index, batch, heads, kv_heads, head_dim, c.format,
                          max_length, int(wp is not None))
     ws = torch.empty(n, dtype=torch.uint8, device=device)
-    _call("mase_paged_attention_decode", device, ctypes.addressof(c), query.data_ptr(), *_strides(query), heads, lp, max_length,
+    _call("mase_paged_attention_decode", device, c.record, query.data_ptr(), *_strides(query), heads, lp, max_length,
           float(scaling), mp, mcode, m_b, wp, w_b, w_h, out.data_ptr(), ws.data_ptr(), n)
     return out
 
@@ -280,19 +306,19 @@ def paged_kv_evict(k_pages: Tensor, v_pages: Tensor, page_table: Tensor, lengths
     ``paged_attention_decode`` and ``paged_kv_append``.  Returns new ``(weights, positions, lengths)``: what belongs to the
     slots now, zero and -1 behind.  A page must belong to one sequence only."""
     what = "paged_kv_evict"
-    c = _pool(what, k_pages, v_pages, page_table, kv_format, k_scales, v_scales,
+    c = _Pool(what, k_pages, v_pages, page_table, kv_format, k_scales, v_scales,
               k_pages.dtype if kv_format is None else torch.bfloat16)
     device = k_pages.device
     keep, recent, first, max_length = int(keep), int(recent), int(first), int(max_length)
     if keep < 1 or recent < 0 or first < 0 or first + recent > keep:
         raise ValueError(f"{what}: keep must be at least 1 and hold first + recent tokens, got keep={keep}, recent={recent}, first={first}")
-    if max_length < 0 or max_length > c.table_pages * c.page_size:
-        raise ValueError(f"{what}: max_length must be between 0 and the table's {c.table_pages * c.page_size} slots, got {max_length}")
+    if max_length < 0 or max_length > c.slots:
+        raise ValueError(f"{what}: max_length must be between 0 and the table's {c.slots} slots, got {max_length}")
     if keep >= max_length:  # no sequence is longer: nothing moves, and no room for moves is needed
         keep, recent, first = max(max_length, 1), 0, 0
     capacity = weights.shape[-1] if weights.dim() == 3 else 0
     shape = (c.batch, c.kv_heads, capacity)
-    if weights.dtype != torch.float32 or tuple(weights.shape) != shape or capacity < max(max_length, 1) or weights.device != device or not weights.is_contiguous():
+    if weights.dtype != torch.float32 or weights.shape != shape or capacity < max(max_length, 1) or weights.device != device or not weights.is_contiguous():
         raise ValueError(f"{what}: weights must be a contiguous float32 tensor [{c.batch}, {c.kv_heads}, at least {max_length}] on {device}")
     pp = _int32(positions, "positions", shape, device)
     lp = _int32(lengths, "lengths", (c.batch,), device)
@@ -300,6 +326,6 @@ def paged_kv_evict(k_pages: Tensor, v_pages: Tensor, page_table: Tensor, lengths
     if c.batch:
         n = _workspace_bytes("mase_paged_kv_evict_workspace_bytes", device.index, c.batch, c.kv_heads, keep)
         ws = torch.empty(n, dtype=torch.uint8, device=device)
-        _call("mase_paged_kv_evict", device, ctypes.addressof(c), lp, max_length, weights.data_ptr(), pp, capacity, keep, recent,
+        _call("mase_paged_kv_evict", device, c.record, lp, max_length, weights.data_ptr(), pp, capacity, keep, recent,
               first, new_weights.data_ptr(), new_positions.data_ptr(), new_lengths.data_ptr(), ws.data_ptr(), n)
     return new_weights, new_positions, new_lengths

@@ -552,6 +552,35 @@ def test_functions_run_on_the_current_stream(dev):
     assert_bits_equal(got, want)
 
 
+def test_calls_on_two_streams_do_not_meet(dev):
+    """two pools worked on at the same time from two streams: the results of one after the other"""
+    jobs = []
+    for i, (lengths, fmt) in enumerate((([3000, 500], "mxint8"), ([2500, 2600], "mxfp4"))):
+        p = Pool(gen(66 + i), lengths, 2, 64, 64, fmt, torch.bfloat16)
+        jobs.append(dict(kw=p.to(dev), n=i32(lengths, dev), top=max(lengths), q=torch.randn(2, 8, 64, generator=gen(68 + i)).bfloat16().to(dev),
+                         pos=torch.arange(p.table.shape[1] * 64, dtype=torch.int32, device=dev).expand(2, 2, -1).contiguous()))
+
+    def work(j):
+        w = torch.zeros(2, 2, j["pos"].shape[2], device=dev)
+        kw = {k: v.clone() if torch.is_tensor(v) else v for k, v in j["kw"].items()}
+        outs = [F().paged_attention_decode(j["q"], **kw, lengths=j["n"], max_length=j["top"], weights=w) for _ in range(5)]
+        w2, pos, n = F().paged_kv_evict(**kw, lengths=j["n"], weights=w, positions=j["pos"], max_length=j["top"], keep=400, recent=9)
+        outs.append(F().paged_attention_decode(j["q"], **kw, lengths=n, max_length=400, weights=w2))
+        return outs + [w2, pos, kw["k_pages"], kw["v_pages"]]
+
+    want = [work(j) for j in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    got = []
+    for s, j in zip(streams, jobs):
+        with torch.cuda.stream(s):
+            got.append(work(j))
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        for x, y in zip(a, b):
+            assert torch.equal(x.view(torch.int16) if x.dtype == torch.bfloat16 else x, y.view(torch.int16) if y.dtype == torch.bfloat16 else y)
+
+
 @pytest.mark.parametrize("fmt", [None, "mxfp8_e5m2"])
 def test_a_step_replays_from_two_graphs(dev, fmt):
     """append + decode with weights captured at two batch layouts; lengths move on inside the graph; replays alternate with
@@ -653,6 +682,7 @@ def test_functions_refuse_what_they_do_not_take(dev):
                 dict(pool=dict(k_scales=None)), dict(pool=dict(k_scales=kw["v_scales"])), dict(pool=dict(kv_format=None)), dict(pool=dict(kv_format="mxfp4")),
                 dict(pool=dict(k_pages=kw["k_pages"][:, :, :8])), dict(pool=dict(v_pages=kw["v_pages"][:1])),
                 dict(pool=dict(page_table=kw["page_table"].long())), dict(pool=dict(page_table=kw["page_table"][:1].expand(2, -1))),
+                dict(pool=dict(k_pages=kw["k_pages"][:1].expand_as(kw["k_pages"]))), dict(pool=dict(v_pages=kw["v_pages"][:, :1].expand_as(kw["v_pages"]))),
                 dict(pool=dict(page_table=kw["page_table"].cpu()))):
         with pytest.raises(ValueError):
             dec(**bad)

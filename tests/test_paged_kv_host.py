@@ -150,6 +150,25 @@ def test_entry_points_refuse_bad_arguments(lib):
     assert evict(ws=None) == -7 and evict(wsb=8) == -7 and evict(ws=p + 4) == -3
 
 
+def test_the_packed_record_is_the_struct():
+    """what the Python functions pack has the layout of mase_paged_kv, field by field"""
+    import struct
+
+    from mase_amd import _lib
+    from mase_amd.quantized.functional import paged_kv
+
+    values = list(range(1, 21))
+    blob = paged_kv._record(*values)
+    assert len(blob) == ctypes.sizeof(_lib.PagedKv) == struct.calcsize("@5P13N2i")
+    c = _lib.PagedKv.from_buffer_copy(blob)
+    assert [getattr(c, n) for n, _ in _lib.PagedKv._fields_] == values
+    text = open(os.path.join(ROOT, "include", "mase_amd.h")).read()
+    body = text[text.index("typedef struct mase_paged_kv {"):text.index("} mase_paged_kv;")]
+    names = [n.strip(" *\n") for line in body.split("{")[1].split(";") for n in line.split("*/")[-1].replace("uint8_t*", "").replace(
+        "const int32_t*", "").replace("void*", "").replace("size_t", "").replace("int32_t", "").split(",") if n.strip(" *\n")]
+    assert names == [n for n, _ in _lib.PagedKv._fields_], names
+
+
 def test_functions_have_no_cpu_path():
     from mase_amd._lib import MaseAmdError
     from mase_amd.quantized import functional as F
