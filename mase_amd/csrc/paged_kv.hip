@@ -92,12 +92,16 @@ __device__ __forceinline__ uint32_t encode8(const uint4& raw, const AppendParams
     const uint32_t m = group_max_u32<4>(vec_absmax_bits<DT>(raw));
     int k = 0, kc = 0;
     const int state = block_exponent<DT>(m, p.mxint, k, kc, meta);
+    // clamp(rint(y)) for the integer bounds is rint(clamp(y)), and adding 1.5 2^23 rounds to the nearest integer, ties to
+    // even, and leaves it in the low byte
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float r = fminf(fmaxf(rintf(ldexpf(x[j], 7 - k)), -128.0f), 127.0f);
-      c[j] = state == 0 ? (uint32_t)(int)r & 0xFFu : 0u;
+    for (int j = 0; j < 8; ++j) c[j] = f2bits(__builtin_amdgcn_fmed3f(ldexpf(x[j], 7 - k), -128.0f, 127.0f) + 12582912.0f);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t lo = __builtin_amdgcn_perm(c[4 * j + 1], c[4 * j], 0x0C0C0400u), hi = __builtin_amdgcn_perm(c[4 * j + 3], c[4 * j + 2], 0x04000C0Cu);
+      w[j] = state == 0 ? lo | hi : 0u;
     }
-    scale = state == 0 ? (uint32_t)(kc + 127) : 255u;  // the quantizer's other blocks are NaN throughout
+    return state == 0 ? (uint32_t)(kc + 127) : 255u;  // the quantizer's other blocks are NaN throughout
   } else {
     constexpr int E = FMT == MASE_KV_MXFP8_E4M3 ? 4 : (FMT == MASE_KV_MXFP8_E5M2 ? 5 : 2), F = FMT == MASE_KV_MXFP8_E4M3 ? 3 : (FMT == MASE_KV_MXFP8_E5M2 ? 2 : 1);
     const uint32_t m = group_max_u32<4>(vec_flushed_absmax<DT>(raw));
@@ -128,34 +132,43 @@ __device__ __forceinline__ uint32_t encode8(const uint4& raw, const AppendParams
   return scale;
 }
 
-// One 16-byte piece (8 elements) of keys and the same of values per lane; consecutive lanes go along the head dimension,
-// then the heads, then the tokens: the order in which projections leave their outputs.  Bound by HBM for prompts (18381
-// tokens, 8 heads of 128 in bf16: 151 MB in 31.6 us), by the launch for single tokens (64 of them: 3 us).
+// One 16-byte piece (8 elements) of keys and the same of values per lane; consecutive lanes go along the head dimension.
+// 16-bit rows: then the heads, then the tokens, the order in which projections leave their outputs (18381 tokens, 8 heads of
+// 128: 151 MB in 32.8 us; the other order 33.9).  Codes: then the tokens, then the heads, so that the scale bytes of the
+// values, which lie slot by slot, meet in a line (9227 tokens in MXINT8, 57 MB: 15.1 us; the other order 16.4).  Bound by
+// HBM for prompts, by the launch for single tokens (64 of them: 3 us).
 template <int D, int FMT, int DT>
 __global__ __launch_bounds__(256) void kv_append_kernel(AppendParams p) {
   constexpr int kPieces = D / 8;
   const int b = blockIdx.y;
   const int count = p.counts == nullptr ? p.tokens : min(p.counts[b], p.tokens);
   const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
-  const uint32_t first_token = (blockIdx.x * 256u) / kPieces / (uint32_t)p.c.heads;
-  if ((int)first_token >= count) return;  // the whole work-group
+  constexpr bool kTokensFirst = FMT != MASE_KV_16BIT;
+  const uint32_t first = (blockIdx.x * 256u) / kPieces;  // of the work-group's rows
+  if constexpr (kTokensFirst) {
+    const uint32_t token = first % (uint32_t)p.tokens;
+    if ((int)token >= count && token + 256u / kPieces <= (uint32_t)p.tokens) return;  // the whole work-group
+  } else {
+    if ((int)(first / (uint32_t)p.c.heads) >= count) return;
+  }
   WaveLog2 meta;
   if constexpr (FMT == MASE_KV_MXINT8) meta.init(p.mxint.tab, 0);
   else if constexpr (FMT != MASE_KV_16BIT) meta.init(p.mxfp.tab, kLog2TabHalf);
   const int piece = (int)(idx % kPieces);
   const uint32_t r = idx / kPieces;
-  const int h = (int)(r % (uint32_t)p.c.heads), j = (int)(r / (uint32_t)p.c.heads);
+  const uint32_t inner = (uint32_t)(kTokensFirst ? p.tokens : p.c.heads);
+  const int in = (int)(r % inner), out = (int)(r / inner);
+  const int j = kTokensFirst ? in : out, h = kTokensFirst ? out : in;
+  // the states are requested before the page is looked up: neither waits for the other
+  uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
   int slot = -1, page = -1;
-  if (idx < p.items) {
+  if (idx < p.items && j < count) {
+    kx = *(const uint4*)(p.key + (size_t)b * p.k_sb + (size_t)h * p.k_sh + (size_t)j * p.k_st + piece * 16);
+    vx = *(const uint4*)(p.value + (size_t)b * p.v_sb + (size_t)h * p.v_sh + (size_t)j * p.v_st + piece * 16);
     slot = kv_new_slot(p.starts[b], count, j, p.c.table_pages, p.c.page_shift);
     page = kv_page(p.c.table + (size_t)b * p.c.table_stride, p.c.table_pages, p.c.page_shift, p.c.num_pages, slot);
   }
   const bool live = page >= 0;
-  uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
-  if (live) {
-    kx = *(const uint4*)(p.key + (size_t)b * p.k_sb + (size_t)h * p.k_sh + (size_t)j * p.k_st + piece * 16);
-    vx = *(const uint4*)(p.value + (size_t)b * p.v_sb + (size_t)h * p.v_sh + (size_t)j * p.v_st + piece * 16);
-  }
   const int row = slot & ((1 << p.c.page_shift) - 1);
   const size_t ko = (size_t)page * p.c.k_page + (size_t)h * p.c.k_head + (size_t)row * p.c.k_slot;
   const size_t vo = (size_t)page * p.c.v_page + (size_t)h * p.c.v_head + (size_t)row * p.c.v_slot;
