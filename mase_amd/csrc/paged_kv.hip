@@ -348,7 +348,7 @@ constexpr int kHeldSlots = 36864;
 
 template <int WAVES, bool HELD>
 __global__ __launch_bounds__(64 * WAVES) void kv_evict_select_kernel(EvictParams p) {
-  constexpr int kThreads = 64 * WAVES, kRun = 8;  // turns whose loads are in flight together
+  constexpr int kThreads = 64 * WAVES, kRun = 8, kFirstRun = 16;  // turns whose loads are in flight together
   extern __shared__ uint32_t held[];              // HELD: [turns * kThreads] keys by slot
   __shared__ __attribute__((aligned(16))) uint32_t hist[256 * kCopies];
   __shared__ int sums[WAVES], sums2[WAVES], found[2];
@@ -373,21 +373,22 @@ __global__ __launch_bounds__(64 * WAVES) void kv_evict_select_kernel(EvictParams
   const int s_lo = wave * turns * 64 + lane;          // this lane's first slot, the next ones 64 apart
   auto there = [&](int k) __attribute__((always_inline)) { return k < turns && s_lo + 64 * k < n; };
 
-  // the largest position; HELD: keys but for the recent slots' protection, which needs it
+  // The largest position; HELD: keys but for the recent slots' protection, which needs it.  Slots behind the last one of the
+  // row have the smallest key, 0: they lie behind every slot that may have it too (NaN), and keep <= n slots come before.
   int newest = -0x7FFFFFFF - 1;
-  for (int k = 0; k < turns; k += kRun) {
-    int pv[kRun];
-    float wv[kRun];
+  for (int k = 0; k < turns; k += kFirstRun) {
+    int pv[kFirstRun];
+    float wv[kFirstRun];
 #pragma unroll
-    for (int j = 0; j < kRun; ++j) {
+    for (int j = 0; j < kFirstRun; ++j) {
       const int s = min(s_lo + 64 * (k + j), n - 1);
       pv[j] = pos[s];
       wv[j] = HELD ? w[s] : 0.0f;
     }
 #pragma unroll
-    for (int j = 0; j < kRun; ++j) {
+    for (int j = 0; j < kFirstRun; ++j) {
       newest = max(newest, pv[j]);
-      if (HELD && k + j < turns) held[s_lo + 64 * (k + j)] = evict_key(wv[j], pv[j], 0x7FFFFFFF, p);
+      if (HELD && k + j < turns) held[s_lo + 64 * (k + j)] = there(k + j) ? evict_key(wv[j], pv[j], 0x7FFFFFFF, p) : 0u;
     }
   }
 #pragma unroll
@@ -404,10 +405,10 @@ __global__ __launch_bounds__(64 * WAVES) void kv_evict_select_kernel(EvictParams
       for (int j = 0; j < kRun; ++j) pv[j] = pos[min(s_lo + 64 * (k + j), n - 1)];
 #pragma unroll
       for (int j = 0; j < kRun; ++j)
-        if (k + j < turns && (long long)pv[j] > (long long)newest - p.recent) held[s_lo + 64 * (k + j)] = 0xFFFFFFFFu;
+        if (there(k + j) && (long long)pv[j] > (long long)newest - p.recent) held[s_lo + 64 * (k + j)] = 0xFFFFFFFFu;
     }
   }
-  // calls f(k, key) for each of this wavefront's turns of 64 slots
+  // calls f(key) for each of this wavefront's turns of 64 slots
   auto for_keys = [&](auto f) __attribute__((always_inline)) {
     if constexpr (HELD) {
       for (int k = 0; k < turns; k += kRun) {
@@ -415,7 +416,8 @@ __global__ __launch_bounds__(64 * WAVES) void kv_evict_select_kernel(EvictParams
 #pragma unroll
         for (int j = 0; j < kRun; ++j) key[j] = held[s_lo + 64 * min(k + j, turns - 1)];
 #pragma unroll
-        for (int j = 0; j < kRun; ++j) f(k + j, key[j]);
+        for (int j = 0; j < kRun; ++j)
+          if (k + j < turns) f(key[j]);
       }
     } else {
       for (int k = 0; k < turns; k += kRun) {
@@ -428,7 +430,8 @@ __global__ __launch_bounds__(64 * WAVES) void kv_evict_select_kernel(EvictParams
           pv[j] = pos[s];
         }
 #pragma unroll
-        for (int j = 0; j < kRun; ++j) f(k + j, evict_key(wv[j], pv[j], newest, p));
+        for (int j = 0; j < kRun; ++j)
+          if (k + j < turns) f(there(k + j) ? evict_key(wv[j], pv[j], newest, p) : 0u);
       }
     }
   };
@@ -436,8 +439,8 @@ __global__ __launch_bounds__(64 * WAVES) void kv_evict_select_kernel(EvictParams
   int want = p.keep;               // how many of the slots with that key are kept: the first ones
 #pragma unroll 1
   for (int shift = 24; shift >= 0; shift -= 8) {
-    for_keys([&](int k, uint32_t key) __attribute__((always_inline)) {
-      if (there(k) && (key & cut_mask) == cut) atomicAdd(&hist[((key >> shift) & 255u) * kCopies + (lane & (kCopies - 1))], 1u);
+    for_keys([&](uint32_t key) __attribute__((always_inline)) {
+      if ((key & cut_mask) == cut) atomicAdd(&hist[((key >> shift) & 255u) * kCopies + (lane & (kCopies - 1))], 1u);
     });
     __syncthreads();
     find_bin(hist, want, sums, found, tid, lane, wave);
@@ -446,9 +449,9 @@ __global__ __launch_bounds__(64 * WAVES) void kv_evict_select_kernel(EvictParams
     cut_mask |= 255u << shift;
   }
   int gt = 0, eq = 0;  // slots above and at the cut: the lane's, the wavefront's, then those before the slot in hand
-  for_keys([&](int k, uint32_t key) __attribute__((always_inline)) {
-    gt += there(k) && key > cut ? 1 : 0;
-    eq += there(k) && key == cut ? 1 : 0;
+  for_keys([&](uint32_t key) __attribute__((always_inline)) {
+    gt += key > cut ? 1 : 0;
+    eq += key == cut ? 1 : 0;
   });
   gt = __builtin_amdgcn_readlane(scan64(gt), 63);
   eq = __builtin_amdgcn_readlane(scan64(eq), 63);
