@@ -340,7 +340,7 @@ __device__ __forceinline__ void find_bin(uint32_t* hist, int want, int* sums, in
 // slot order come from counts per wavefront and ballots within it.  The key of the keep-th largest slot is found by four
 // histograms over 8 bits of the keys each.  HELD: the row's keys stay in LDS (rows of up to kHeldSlots); otherwise
 // they are made anew from L2 for each pass.
-// It is bound by the latency of its dependent steps on one CU (two reads of the row, four histograms, the ranks): 42 us for
+// It is bound by the latency of its dependent steps on one CU (two reads of the row, four histograms, the ranks): 39 us for
 // 64 rows of 20001 .. 32768 slots, 11 us for 8 rows of 2047.  Weights and positions are read in runs of independent loads
 // (one at a time, each waiting for L2: 103 us); keys in registers with every turn unrolled were no faster (45 us: the code
 // itself came from memory).
