@@ -18,7 +18,8 @@ What is quantized (``q_config`` sub-dicts, each with an optional ``bypass``):
   ``softmax``   the masked scores, minifloat cast, softmax in fp32    (attention.py:369-375)
   ``av_matmul`` the probabilities (not the values) along the key axis (attention.py:383-392)
 With a ``PagedKVCache`` as ``past_key_value``, a step of one new token with ``softmax`` and ``av_matmul`` bypassed is
-attended from the pages (no attention weights are returned); other steps read the cache back dense.
+attended from the pages (no attention weights are returned); other steps read the cache back dense.  Columns of the mask
+are positions, also after an eviction, which leaves fewer slots than positions in an order of its own for each cached head.
 MLP: ``silu_minifloat`` on the gate projection (mlp.py:60-62, 75-77); RMSNorm: minifloat cast of the input and of the
 weight (rms_norm.py:72-84).
 """
@@ -189,6 +190,7 @@ class _LlamaAttentionMX(nn.Module):
             paged = isinstance(past_key_value, PagedKVCache)
             if paged:
                 past_key_value.require_kind(None if self.kv_cache_bypass else self._kind, self.kv_cache_config)
+                past_key_value.require_mask(attention_mask, query_states.shape[2], self.layer_idx)
                 if self._reads_pages(query_states, attention_mask):
                     return self._attend_pages(past_key_value, query_states, key_states, value_states, attention_mask, input_shape)
             # a packed paged cache quantizes what it writes
@@ -196,6 +198,8 @@ class _LlamaAttentionMX(nn.Module):
                 kv_cache = kv_cache_mxfp if self._kind == "mxfp" else kv_cache_mxint
                 key_states, value_states = kv_cache(key_states, value_states, self.kv_cache_config)
             key_states, value_states = past_key_value.update(key_states, value_states, self.layer_idx, cache_kwargs)
+            if paged:
+                attention_mask = past_key_value.slot_mask(attention_mask, query_states.shape[1], self.layer_idx)
 
         attn_output, attn_weights = _eager_attention_forward(
             self._kind, self, query_states, key_states, value_states, attention_mask,

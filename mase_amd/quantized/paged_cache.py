@@ -102,6 +102,43 @@ class PagedKVCache:
         if config["data_in_block_size"] != 32 or _FORMAT_OF.get((kind, *bits)) != self.kv_format:
             raise ValueError(f"a PagedKVCache of {self.kv_format} codes does not hold the values of the module's kv_cache quantizer ({kind}, {config}): use kv_format=None")
 
+    # -- masks --------------------------------------------------------------------------------------------------------
+    # A mask of a step has one column for each position, as the callers of the attention modules make it.  Until a layer is
+    # evicted from, slots are positions; afterwards every cached head has an order of slots of its own.
+    def _evicted(self, layer: int) -> bool:
+        return self._held[layer] != self._seen[layer]
+
+    def require_mask(self, mask: Optional[Tensor], tokens: int, layer_idx: int = 0) -> None:
+        """raises ValueError unless ``mask`` (``[batch or 1, heads or 1, tokens or 1, columns]``, added to the scores of the
+        next ``tokens`` tokens, one column for each position) can be laid over the layer's slots once they are appended"""
+        evicted = self._evicted(layer_idx)
+        if mask is None or not (evicted or tokens == 1):  # the dense chain's own business
+            return
+        total = self.get_seq_length(layer_idx) + tokens
+        fits = mask.dim() == 4 and mask.shape[0] in (1, self.batch_size) and mask.shape[3] >= total
+        if fits and evicted:
+            fits = mask.is_floating_point() and mask.shape[2] in (1, tokens) and (mask.shape[1] == 1 or mask.shape[1] % self.num_kv_heads == 0)
+        if not fits:
+            raise ValueError(f"mask must be a floating-point tensor [{self.batch_size} or 1, heads or 1, {tokens} or 1, at least {total}] with "
+                             f"one column for each position, got {mask.dtype} {tuple(mask.shape)}")
+
+    def slot_mask(self, mask: Optional[Tensor], heads: int, layer_idx: int = 0) -> Optional[Tensor]:
+        """the mask over the rows that ``gather`` returns, of one whose columns are positions: the same one until the layer
+        is evicted from, then ``[batch, heads, rows, longest]``"""
+        if mask is None or not self._evicted(layer_idx):
+            return mask
+        batch, rows, columns = self.batch_size, mask.shape[2], mask.shape[3]
+        # the query heads of a cached head see the same slots: one row of columns for all of them where the mask has one
+        group = heads // self.num_kv_heads if mask.shape[1] > 1 else 1
+        at = self._slot_positions(layer_idx)[:, :, None, None]
+        by_head = mask.expand(batch, group * self.num_kv_heads, rows, columns).unflatten(1, (self.num_kv_heads, group))
+        got = by_head.gather(-1, at.expand(-1, -1, group, rows, -1))
+        return got.expand(-1, -1, heads // self.num_kv_heads, -1, -1).flatten(1, 2)
+
+    def _slot_positions(self, layer: int) -> Tensor:
+        """int64 ``[batch, kv_heads, longest]``; 0 for slots behind a sequence's last one, which no kernel looks at"""
+        return self._positions[layer][:, :, :max(self._held[layer])].clamp(min=0).long()
+
     # -- a step -------------------------------------------------------------------------------------------------------
     def append(self, key_states: Tensor, value_states: Tensor, layer_idx: int = 0, counts: Optional[Sequence[int]] = None) -> None:
         """adds ``[batch, kv_heads, tokens, head_dim]`` states behind what the layer holds; ``counts[b]`` of the tokens for
@@ -136,10 +173,40 @@ class PagedKVCache:
                                  **self._codes(layer_idx))
 
     def attend(self, query: Tensor, layer_idx: int = 0, *, scaling: Optional[float] = None, mask: Optional[Tensor] = None) -> Tensor:
-        """attention of one token per sequence, ``[batch, heads, head_dim]``, over what the layer holds"""
+        """attention of one token per sequence, ``[batch, heads, head_dim]``, over what the layer holds.  ``mask``
+        (``[batch or 1, (1, ...) columns]`` of the states' type or float32): column c is added to the scores of the token at
+        position c of its sequence, wherever an eviction has put it"""
+        if mask is not None and self._evicted(layer_idx):
+            return self._attend_by_position(query, layer_idx, scaling, mask)
         return F.paged_attention_decode(query, *self._pool(layer_idx), self._held_dev[layer_idx], max(self._held[layer_idx]),
                                         scaling=scaling, mask=mask, weights=self._weights[layer_idx] if self.track_weights else None,
                                         **self._codes(layer_idx))
+
+    def _attend_by_position(self, query: Tensor, layer: int, scaling: Optional[float], mask: Tensor) -> Tensor:
+        """``attend`` with a mask after an eviction: each cached head of a sequence has its own order of slots, so it becomes
+        a sequence of one head, with its own mask row, in a pool whose pages are the heads of the pages"""
+        batch, heads, columns = self.batch_size, self.num_kv_heads, max(self._seen[layer])
+        if (mask.dim() < 2 or mask.shape[0] not in (1, batch) or any(n != 1 for n in mask.shape[1:-1]) or mask.shape[-1] < columns
+                or mask.dtype not in (self.dtype, torch.float32)):
+            raise ValueError(f"mask must be {self.dtype} or float32 [{batch} or 1, (1, ...) at least {columns}] with one column for each "
+                             f"position, got {mask.dtype} {tuple(mask.shape)}")
+        if query.dim() != 3 or query.shape[0] != batch or query.shape[1] % heads:
+            raise ValueError(f"query must be [{batch}, a multiple of {heads}, {self.head_dim}], got {tuple(query.shape)}")
+        if batch * heads > 65535:
+            raise ValueError(f"a mask after an eviction is for at most 65535 cached heads of sequences, got {batch * heads}")
+        flat = mask.reshape(mask.shape[0], 1, mask.shape[-1]).expand(batch, heads, -1)
+        rows = flat.gather(-1, self._slot_positions(layer)).flatten(0, 1)
+        single = lambda t: t.flatten(0, 1).unsqueeze(1)  # noqa: E731  [pages, heads, ...] as [pages * heads, 1, ...]
+        head = torch.arange(heads, dtype=torch.int32, device=self.device)[:, None]
+        table = torch.where(self._table[:, None] < 0, -1, self._table[:, None] * heads + head).flatten(0, 1)
+        lengths = self._held_dev[layer].repeat_interleave(heads)
+        codes = self._codes(layer)
+        if codes:
+            codes.update(k_scales=single(codes["k_scales"]), v_scales=single(codes["v_scales"]))
+        out = F.paged_attention_decode(query.reshape(batch * heads, -1, query.shape[2]), single(self._k[layer]), single(self._v[layer]),
+                                       table, lengths, max(self._held[layer]), scaling=scaling, mask=rows,
+                                       weights=single(self._weights[layer]), **codes)
+        return out.view(query.shape)
 
     # -- room ---------------------------------------------------------------------------------------------------------
     def evict(self, keep: int, *, recent: int = 0, first: int = 0) -> None:

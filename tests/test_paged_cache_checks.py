@@ -1,0 +1,62 @@
+"""PagedKVCache on the host: masks over positions laid over slots, and what is refused before anything changes."""
+import pytest
+import torch
+
+
+def cache(held, seen, positions=None, heads=2, capacity=32, dtype=torch.bfloat16):
+    """a cache on the CPU that holds `held` of the `seen` tokens of each sequence at the given positions"""
+    from mase_amd.quantized import PagedKVCache
+
+    c = PagedKVCache(len(held), heads, 64, capacity, page_size=16, dtype=dtype, device="cpu", track_weights=True)
+    c._held, c._seen = [list(held)], [list(seen)]
+    c._held_dev[0], c._seen_dev[0] = torch.tensor(held, dtype=torch.int32), torch.tensor(seen, dtype=torch.int32)
+    if positions is not None:
+        c._positions[0] = positions
+    return c
+
+
+def scattered(held, seen, heads, capacity, gen):
+    """an order of slots of its own for each head"""
+    pos = torch.full((len(held), heads, capacity), -1, dtype=torch.int32)
+    for b, (n, total) in enumerate(zip(held, seen)):
+        for h in range(heads):
+            pos[b, h, :n] = torch.randperm(total, generator=gen)[:n].to(torch.int32)
+    return pos
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape", [(1, 1, 3, 24), (2, 1, 3, 24), (2, 6, 3, 24), (2, 1, 1, 24), (1, 6, 1, 40)])
+def test_columns_of_positions_become_columns_of_slots(shape, dtype):
+    g = torch.Generator().manual_seed(110)
+    pos = scattered([10, 10], [24, 24], 2, 32, g)
+    c = cache([10, 10], [24, 24], pos)
+    mask = torch.randn(shape, generator=g).to(dtype)
+    got = c.slot_mask(mask, 6)
+    assert got.dtype == dtype and got.shape == (2, 6, shape[2], 10)
+    for b in range(2):
+        for h in range(6):
+            for t in range(shape[2]):
+                for s in range(10):
+                    want = mask[b if shape[0] > 1 else 0, h if shape[1] > 1 else 0, t, int(pos[b, h // 3, s])]
+                    assert got[b, h, t, s] == want
+
+
+def test_masks_stay_as_they_are_until_a_layer_is_evicted_from():
+    c = cache([10, 10], [10, 10])
+    mask = torch.zeros(2, 1, 3, 13)
+    c.require_mask(mask, 3)
+    assert c.slot_mask(mask, 6) is mask and c.slot_mask(None, 6) is None
+    c.require_mask(torch.zeros(2, 1, 1, 11, dtype=torch.bool), 1)  # the dense chain's own business
+    with pytest.raises(ValueError, match="mask"):
+        c.require_mask(torch.zeros(2, 1, 1, 10), 1)
+
+
+@pytest.mark.parametrize("bad", [torch.zeros(2, 1, 3, 26), torch.zeros(2, 1, 2, 27), torch.zeros(3, 1, 3, 27), torch.zeros(2, 3, 3, 27),
+                                 torch.zeros(2, 3, 27), torch.zeros(2, 1, 3, 27, dtype=torch.bool)])
+def test_masks_that_are_no_masks_of_positions_are_refused_after_an_eviction(bad):
+    c = cache([10, 10], [24, 24])
+    c.require_mask(torch.zeros(2, 1, 3, 27), 3)
+    c.require_mask(torch.zeros(1, 6, 1, 40), 3)
+    c.require_mask(None, 3)
+    with pytest.raises(ValueError, match="mask"):
+        c.require_mask(bad, 3)
