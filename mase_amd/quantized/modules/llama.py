@@ -19,7 +19,8 @@ What is quantized (``q_config`` sub-dicts, each with an optional ``bypass``):
   ``av_matmul`` the probabilities (not the values) along the key axis (attention.py:383-392)
 With a ``PagedKVCache`` as ``past_key_value``, a step of one new token with ``softmax`` and ``av_matmul`` bypassed is
 attended from the pages (no attention weights are returned); other steps read the cache back dense.  Columns of the mask
-are positions, also after an eviction, which leaves fewer slots than positions in an order of its own for each cached head.
+are positions, also after an eviction, which leaves fewer slots than positions in an order of its own for each cached
+head; sequences that have seen different numbers of tokens take steps without a mask only.
 MLP: ``silu_minifloat`` on the gate projection (mlp.py:60-62, 75-77); RMSNorm: minifloat cast of the input and of the
 weight (rms_norm.py:72-84).
 """

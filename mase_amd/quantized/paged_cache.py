@@ -111,7 +111,10 @@ class PagedKVCache:
     def require_mask(self, mask: Optional[Tensor], tokens: int, layer_idx: int = 0) -> None:
         """raises ValueError unless ``mask`` (``[batch or 1, heads or 1, tokens or 1, columns]``, added to the scores of the
         next ``tokens`` tokens, one column for each position) can be laid over the layer's slots once they are appended"""
-        evicted = self._evicted(layer_idx)
+        evicted, seen = self._evicted(layer_idx), self._seen[layer_idx]
+        if mask is not None and min(seen) != max(seen):
+            raise ValueError("a mask with one column for each position needs sequences that stand at the same one: these have seen "
+                             f"{min(seen)} to {max(seen)} tokens (steps without a mask and attend() with one take such sequences)")
         if mask is None or not (evicted or tokens == 1):  # the dense chain's own business
             return
         total = self.get_seq_length(layer_idx) + tokens
@@ -124,9 +127,19 @@ class PagedKVCache:
 
     def slot_mask(self, mask: Optional[Tensor], heads: int, layer_idx: int = 0) -> Optional[Tensor]:
         """the mask over the rows that ``gather`` returns, of one whose columns are positions: the same one until the layer
-        is evicted from, then ``[batch, heads, rows, longest]``"""
-        if mask is None or not self._evicted(layer_idx):
+        is evicted from, then ``[batch, heads, rows, longest]``.  The zeros behind shorter sequences are hidden by the type's
+        lowest value (without a mask: by one of the states' type, ``[batch, 1, 1, longest]``)"""
+        held = self._held[layer_idx]
+        if mask is not None and self._evicted(layer_idx):
+            mask = self._gather_columns(mask, heads, layer_idx)
+        if min(held) == max(held):
             return mask
+        if mask is None:
+            mask = torch.zeros((self.batch_size, 1, 1, max(held)), dtype=self.dtype, device=self.device)
+        behind = torch.arange(max(held), device=self.device) >= self._held_dev[layer_idx][:, None]
+        return mask[..., :max(held)].masked_fill(behind[:, None, None], torch.finfo(mask.dtype).min)
+
+    def _gather_columns(self, mask: Tensor, heads: int, layer_idx: int) -> Tensor:
         batch, rows, columns = self.batch_size, mask.shape[2], mask.shape[3]
         # the query heads of a cached head see the same slots: one row of columns for all of them where the mask has one
         group = heads // self.num_kv_heads if mask.shape[1] > 1 else 1

@@ -60,3 +60,30 @@ def test_masks_that_are_no_masks_of_positions_are_refused_after_an_eviction(bad)
     c.require_mask(None, 3)
     with pytest.raises(ValueError, match="mask"):
         c.require_mask(bad, 3)
+
+
+@pytest.mark.parametrize("evicted", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_rows_behind_shorter_sequences_are_hidden(dtype, evicted):
+    held, seen = [10, 4, 7], [24, 24, 24] if evicted else [10, 4, 7]
+    g = torch.Generator().manual_seed(111)
+    c = cache(held, seen, scattered(held, seen, 2, 32, g), dtype=dtype)
+    behind = torch.arange(10) >= torch.tensor(held)[:, None]
+    got = c.slot_mask(None, 6)
+    assert got.dtype == dtype and got.shape == (3, 1, 1, 10)
+    assert bool((got[:, 0, 0][behind] == torch.finfo(dtype).min).all()) and not bool(got[:, 0, 0][~behind].any())
+    if evicted:
+        mask = torch.randn(3, 1, 2, 24, generator=g)
+        got = c.slot_mask(mask, 6)
+        for b in range(3):
+            assert bool((got[b, :, :, behind[b]] == torch.finfo(torch.float32).min).all())
+            for h in range(6):
+                assert torch.equal(got[b, h, :, :held[b]], mask[b, 0][:, c._positions[0][b, h // 3, :held[b]].long()])
+
+
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_masks_need_sequences_that_stand_at_one_position(tokens):
+    c = cache([10, 4], [10, 4])
+    c.require_mask(None, tokens)
+    with pytest.raises(ValueError, match="4 to 10 tokens"):
+        c.require_mask(torch.zeros(2, 1, tokens, 10 + tokens), tokens)

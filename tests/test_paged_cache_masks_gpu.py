@@ -191,3 +191,32 @@ def test_a_refused_mask_leaves_the_cache_as_it_was(dev):
         refused(3, 20, position_mask(3, 23, dev).expand(2, 3, 3, 23))  # neither one head nor all of them
         for n in (1, 3):                                             # these fit
             m(x[:, :n], tables(n, 64, 20, dev, DTYPE), position_mask(n, cache.get_seq_length() + n, dev), past_key_value=cache)
+
+
+@pytest.mark.parametrize("evicted", [False, True])
+def test_dense_steps_of_unequal_sequences_see_only_their_own_slots(dev, evicted):
+    """several tokens at once, without a mask, on a cache whose sequences hold different numbers of slots"""
+    m, cache = module(dev), make(dev)
+    kv = torch.randn(2, 2, 4, 30, 64, generator=torch.Generator().manual_seed(75)).to(DTYPE).to(dev)
+    cache.append(kv[0], kv[1], counts=[30, 9])
+    if evicted:
+        cache.evict(14, recent=4)
+    x = torch.randn(2, 2, 256, generator=torch.Generator().manual_seed(76)).to(DTYPE).to(dev)
+    cos_sin = tables(2, 64, 9, dev, DTYPE)
+    with torch.no_grad():
+        y, _ = m(x, cos_sin, None, past_key_value=cache)
+    assert cache.lengths(0) == [16 if evicted else 32, 11]
+    check_step(m, cache, dict(x=x, cos_sin=cos_sin, y=y, n=2, mask=torch.zeros(2, 1, 2, 32)))
+
+
+def test_masks_of_positions_are_refused_where_sequences_stand_at_different_ones(dev):
+    """a column cannot be one position of all sequences for the new tokens; nothing is appended"""
+    m, cache = module(dev), make(dev)
+    kv = torch.randn(2, 2, 4, 30, 64, generator=torch.Generator().manual_seed(77)).to(DTYPE).to(dev)
+    cache.append(kv[0], kv[1], counts=[30, 9])
+    x = torch.randn(2, 3, 256, generator=torch.Generator().manual_seed(78)).to(DTYPE).to(dev)
+    with torch.no_grad():
+        for n in (1, 3):
+            with pytest.raises(ValueError, match="mask"):
+                m(x[:, :n], tables(n, 64, 30, dev, DTYPE), position_mask(n, 30 + n, dev, pads=(0, 0)), past_key_value=cache)
+    assert cache.lengths(0) == [30, 9]
