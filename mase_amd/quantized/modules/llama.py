@@ -207,6 +207,8 @@ class _LlamaAttentionMX(nn.Module):
             dropout=0.0 if not self.training else self.attention_dropout, scaling=self.scaling,
             qk_bypass=self.qk_bypass, qk_config=self.qk_config, av_bypass=self.av_bypass, av_config=self.av_config,
             softmax_bypass=self.softmax_bypass, softmax_config=self.softmax_config, **kwargs)
+        if past_key_value is not None and paged and past_key_value.track_weights:
+            past_key_value.add_weights(attn_weights, self.layer_idx, attention_mask)
         attn_output = attn_output.reshape(*input_shape, -1).contiguous()
         attn_output = self.o_proj(attn_output)
         return attn_output, attn_weights

@@ -26,8 +26,9 @@ class PagedKVCache:
 
     ``kv_format``: None (states of ``dtype``), ``"mxint8"``, ``"mxfp8_e4m3"``, ``"mxfp8_e5m2"`` or ``"mxfp4"`` (blocks of 32
     along the head dimension).  ``num_pages`` (default: enough for every sequence at ``max_length``) is the pool's size for
-    each layer; a sequence takes pages as it grows.  ``track_weights``: ``attend`` adds up the attention weights and
-    positions are kept, which ``evict`` needs."""
+    each layer; a sequence takes pages as it grows.  ``track_weights``: positions and the
+    sums of the attention weights are kept, which ``evict`` needs; ``attend`` adds to them, and so do the attention modules'
+    dense steps (``add_weights``)."""
 
     def __init__(self, batch_size: int, num_kv_heads: int, head_dim: int, max_length: int, num_layers: int = 1, *,
                  page_size: int = 64, num_pages: Optional[int] = None, kv_format: Optional[str] = None,
@@ -194,6 +195,23 @@ class PagedKVCache:
         return F.paged_attention_decode(query, *self._pool(layer_idx), self._held_dev[layer_idx], max(self._held[layer_idx]),
                                         scaling=scaling, mask=mask, weights=self._weights[layer_idx] if self.track_weights else None,
                                         **self._codes(layer_idx))
+
+    def add_weights(self, probabilities: Tensor, layer_idx: int = 0, mask: Optional[Tensor] = None) -> None:
+        """adds the attention probabilities ``[batch, heads, tokens, longest]`` of a step that was computed on what ``update``
+        returned to the weights that ``evict`` ranks by, summed over tokens and the query heads of each cached head (``attend``
+        does so itself).  ``mask``: the one of that step; tokens whose row of it hides every slot are padding and do not count"""
+        self._require_tracking("add_weights")
+        longest = max(self._held[layer_idx])
+        shape = tuple(probabilities.shape)
+        if len(shape) != 4 or shape[0] != self.batch_size or shape[1] % self.num_kv_heads or shape[1] == 0 or shape[3] != longest:
+            raise ValueError(f"probabilities must be [{self.batch_size}, a multiple of {self.num_kv_heads}, tokens, {longest}], got {shape}")
+        p = probabilities.detach()
+        if mask is not None and mask.is_floating_point() and shape[2] > 1:
+            # half the lowest value: masks are also made by adding two of them up
+            padding = mask[..., :longest].amax(-1, keepdim=True) <= torch.finfo(mask.dtype).min / 2
+            p = p.masked_fill(padding, 0.0)
+        by_head = p.unflatten(1, (self.num_kv_heads, -1))
+        self._weights[layer_idx][:, :, :longest] += by_head.sum((2, 3), dtype=torch.float32)
 
     def _attend_by_position(self, query: Tensor, layer: int, scaling: Optional[float], mask: Tensor) -> Tensor:
         """``attend`` with a mask after an eviction: each cached head of a sequence has its own order of slots, so it becomes
