@@ -165,7 +165,7 @@ class PagedKVCache:
             raise ValueError(f"counts must be {self.batch_size} numbers from 0 to {n}, got {new}")
         held, seen = self._held[layer_idx], self._seen[layer_idx]
         self._grow([h + c for h, c in zip(held, new)])
-        counts_dev = None if counts is None else torch.tensor(new, dtype=torch.int32, device=self.device)
+        counts_dev = None if counts is None else self._staged(new).to(torch.int32)
         track = dict(positions=self._positions[layer_idx], first_positions=self._seen_dev[layer_idx]) if self.track_weights else {}
         F.paged_kv_append(key_states, value_states, *self._pool(layer_idx), self._held_dev[layer_idx], counts=counts_dev, **track,
                           **self._codes(layer_idx))
@@ -305,5 +305,11 @@ class PagedKVCache:
 
     def _set_table(self, at, pages) -> None:
         if at:
-            rows, cols = torch.tensor(at, device=self.device).unbind(1)
-            self._table[rows, cols] = torch.tensor(pages, dtype=torch.int32, device=self.device)
+            rows, cols, numbers = self._staged([(b, i, page) for (b, i), page in zip(at, pages)]).unbind(1)
+            self._table[rows, cols] = numbers.to(torch.int32)
+
+    def _staged(self, values) -> Tensor:
+        """int64 numbers of the host on the device, in the order of the stream: a copy from pageable memory would wait for the
+        GPU.  torch's allocator of pinned memory does not hand a block out again before the copies from it are done"""
+        host = torch.tensor(values, dtype=torch.int64, pin_memory=self.device.type == "cuda")
+        return host.to(self.device, non_blocking=True)
