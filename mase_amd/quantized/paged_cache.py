@@ -5,8 +5,8 @@ It takes the place of the cache object that the attention modules call ``past_ke
 ``attend`` do a decoding step on the pages alone, and ``evict`` cuts the sequences down to a budget by the attention
 weights that ``attend`` has added up.  The functions underneath are in ``mase_amd.quantized.functional``.
 
-The host keeps how long each sequence is, so no call waits for the GPU; a step that is captured into a graph uses the
-functions directly, with lengths that the graph itself moves on.
+The host keeps how long each sequence is, so no call waits for the GPU; a replayed graph would not move that on, so no
+call can be captured: a step that is captured uses the functions directly, with lengths that the graph itself moves on.
 """
 from __future__ import annotations
 
@@ -15,6 +15,7 @@ from typing import List, Optional, Sequence, Tuple
 import torch
 from torch import Tensor
 
+from .. import _lib
 from .functional import paged_kv as F
 
 # (kind, element bits or exponent and fraction bits) of the kv_cache quantizer that each code format holds the values of
@@ -159,6 +160,7 @@ class PagedKVCache:
         sequence b where given (a padded batch)"""
         if key_states.dim() != 4 or key_states.shape[0] != self.batch_size or key_states.dtype != self.dtype:
             raise ValueError(f"states must be {self.dtype} [{self.batch_size}, {self.num_kv_heads}, tokens, {self.head_dim}], got {key_states.dtype} {tuple(key_states.shape)}")
+        self._refuse_capture("append")
         n = key_states.shape[2]
         new = [n] * self.batch_size if counts is None else [int(c) for c in counts]
         if len(new) != self.batch_size or any(c < 0 or c > n for c in new):
@@ -183,6 +185,7 @@ class PagedKVCache:
         return self.gather(layer_idx)
 
     def gather(self, layer_idx: int = 0) -> Tuple[Tensor, Tensor]:
+        self._refuse_capture("gather")
         return F.paged_kv_gather(*self._pool(layer_idx), self._held_dev[layer_idx], max(self._held[layer_idx]), dtype=self.dtype,
                                  **self._codes(layer_idx))
 
@@ -190,6 +193,7 @@ class PagedKVCache:
         """attention of one token per sequence, ``[batch, heads, head_dim]``, over what the layer holds.  ``mask``
         (``[batch or 1, (1, ...) columns]`` of the states' type or float32): column c is added to the scores of the token at
         position c of its sequence, wherever an eviction has put it"""
+        self._refuse_capture("attend")
         if mask is not None and self._evicted(layer_idx):
             return self._attend_by_position(query, layer_idx, scaling, mask)
         return F.paged_attention_decode(query, *self._pool(layer_idx), self._held_dev[layer_idx], max(self._held[layer_idx]),
@@ -201,6 +205,7 @@ class PagedKVCache:
         returned to the weights that ``evict`` ranks by, summed over tokens and the query heads of each cached head (``attend``
         does so itself).  ``mask``: the one of that step; tokens whose row of it hides every slot are padding and do not count"""
         self._require_tracking("add_weights")
+        self._refuse_capture("add_weights")
         longest = max(self._held[layer_idx])
         shape = tuple(probabilities.shape)
         if len(shape) != 4 or shape[0] != self.batch_size or shape[1] % self.num_kv_heads or shape[1] == 0 or shape[3] != longest:
@@ -244,6 +249,7 @@ class PagedKVCache:
         """cuts every sequence down to ``keep`` tokens in every layer and cached head (see ``paged_kv_evict``) and gives the
         pages behind them back; between steps, when all layers hold the same tokens"""
         self._require_tracking("evict")
+        self._refuse_capture("evict")
         if any(h != self._held[0] for h in self._held):
             raise ValueError("evict() comes between steps: the layers do not hold the same number of tokens")
         longest = max(self._held[0])
@@ -266,6 +272,7 @@ class PagedKVCache:
 
     def reset(self) -> None:
         """forgets every sequence"""
+        self._refuse_capture("reset")
         self._free = list(range(self.num_pages - 1, -1, -1))
         self._pages = [[] for _ in range(self.batch_size)]
         self._held, self._seen = ([[0] * self.batch_size for _ in range(self.num_layers)] for _ in range(2))
@@ -279,6 +286,11 @@ class PagedKVCache:
     def _require_tracking(self, what: str) -> None:
         if not self.track_weights:
             raise ValueError(f"{what} needs a cache made with track_weights=True")
+
+    def _refuse_capture(self, what: str) -> None:
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise _lib.MaseAmdError(f"PagedKVCache.{what} cannot be captured into a graph, which would not move the lengths on the host: "
+                                    "capture the functions of mase_amd.quantized.functional instead")
 
     def _pool(self, layer: int):
         return self._k[layer], self._v[layer], self._table

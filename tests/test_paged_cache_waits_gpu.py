@@ -1,4 +1,4 @@
-"""What a PagedKVCache does on the host: no call waits for the GPU."""
+"""What a PagedKVCache does on the host: no call waits for the GPU, and none can be captured."""
 import pytest
 import torch
 
@@ -58,3 +58,27 @@ def test_staged_page_numbers_arrive_in_order(dev):
     assert torch.equal(c._table, d._table) and c._held_dev[0].tolist() == c.lengths() == [35, 33]
     for a, b in zip(c.gather(), d.gather()):
         assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+
+
+def test_steps_refuse_to_be_captured(dev):
+    """a replay would not move the host's lengths on"""
+    c = make(dev)
+    x = torch.randn(2, 2, 4, 64, generator=torch.Generator().manual_seed(93)).bfloat16().to(dev)
+    q = torch.randn(2, 4, 64, generator=torch.Generator().manual_seed(94)).bfloat16().to(dev)
+    c.update(x, x)
+    want = c.attend(q)
+    other = torch.zeros(8, device=dev)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        other += 1
+        for call in (lambda: c.append(x, x), lambda: c.update(x, x), lambda: c.gather(), lambda: c.attend(q),
+                     lambda: c.add_weights(torch.empty(2, 2, 1, 4, device=dev)), lambda: c.evict(2), lambda: c.reset()):
+            with pytest.raises(RuntimeError, match="captured"):
+                call()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert c.lengths() == [4, 4] and other.tolist() == [1.0] * 8
+    c.reset()
+    c.update(x, x)
+    assert torch.equal(c.attend(q), want)
