@@ -166,14 +166,23 @@ class PagedKVCache:
         if len(new) != self.batch_size or any(c < 0 or c > n for c in new):
             raise ValueError(f"counts must be {self.batch_size} numbers from 0 to {n}, got {new}")
         held, seen = self._held[layer_idx], self._seen[layer_idx]
+        before = [len(p) for p in self._pages]
         self._grow([h + c for h, c in zip(held, new)])
-        counts_dev = None if counts is None else self._staged(new).to(torch.int32)
-        track = dict(positions=self._positions[layer_idx], first_positions=self._seen_dev[layer_idx]) if self.track_weights else {}
-        F.paged_kv_append(key_states, value_states, *self._pool(layer_idx), self._held_dev[layer_idx], counts=counts_dev, **track,
-                          **self._codes(layer_idx))
+        try:
+            self._write(key_states, value_states, layer_idx, n, None if counts is None else new)
+        except Exception:
+            self._give_back(before)  # a call that is refused takes no pages
+            raise
         for b, c in enumerate(new):
             held[b] += c
             seen[b] += c
+
+    def _write(self, key_states: Tensor, value_states: Tensor, layer_idx: int, n: int, new: Optional[List[int]]) -> None:
+        """the states into their pages, and the lengths on the device moved on"""
+        counts_dev = None if new is None else self._staged(new).to(torch.int32)
+        track = dict(positions=self._positions[layer_idx], first_positions=self._seen_dev[layer_idx]) if self.track_weights else {}
+        F.paged_kv_append(key_states, value_states, *self._pool(layer_idx), self._held_dev[layer_idx], counts=counts_dev, **track,
+                          **self._codes(layer_idx))
         step = n if counts_dev is None else counts_dev
         self._held_dev[layer_idx] += step
         self._seen_dev[layer_idx] += step
@@ -262,13 +271,7 @@ class PagedKVCache:
             self._positions[layer].copy_(pos)
             self._held_dev[layer].copy_(n)
             self._held[layer] = [min(h, keep) for h in self._held[layer]]
-        dropped = []
-        for b, pages in enumerate(self._pages):
-            left = -(-self._held[0][b] // self.page_size)
-            dropped += [(b, i) for i in range(left, len(pages))]
-            self._free += reversed(pages[left:])
-            del pages[left:]
-        self._set_table(dropped, [-1] * len(dropped))
+        self._give_back([-(-h // self.page_size) for h in self._held[0]])
 
     def reset(self) -> None:
         """forgets every sequence"""
@@ -314,6 +317,16 @@ class PagedKVCache:
                 got.append(self._free.pop())
                 self._pages[b].append(got[-1])
         self._set_table(at, got)
+
+    def _give_back(self, left: Sequence[int]) -> None:
+        """the pages of each sequence behind its first left[b]"""
+        dropped = []
+        for b in range(self.batch_size - 1, -1, -1):  # the last one taken first
+            pages, n = self._pages[b], left[b]
+            dropped += [(b, i) for i in range(n, len(pages))]
+            self._free += reversed(pages[n:])
+            del pages[n:]
+        self._set_table(dropped, [-1] * len(dropped))
 
     def _set_table(self, at, pages) -> None:
         if at:

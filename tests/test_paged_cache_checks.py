@@ -87,3 +87,20 @@ def test_masks_need_sequences_that_stand_at_one_position(tokens):
     c.require_mask(None, tokens)
     with pytest.raises(ValueError, match="4 to 10 tokens"):
         c.require_mask(torch.zeros(2, 1, tokens, 10 + tokens), tokens)
+
+
+def test_a_refused_append_takes_no_pages():
+    """states that the functions refuse (here: no GPU, other shapes) leave pages, table and lengths as they were"""
+    from mase_amd._lib import MaseAmdError
+    from mase_amd.quantized import PagedKVCache
+
+    c = PagedKVCache(2, 1, 64, 100, page_size=16, num_pages=7, device="cpu")
+    c._grow([17, 0])
+    c._held[0][0] = 17
+    free, table = list(c._free), c._table.clone()
+    x = torch.zeros(2, 1, 30, 64, dtype=torch.bfloat16)
+    for key, value, counts in ((x, x, None), (x, x, [30, 0]), (x.expand(2, 2, 30, 64), x, None), (x, x[:, :, :4], None), (x[..., :32], x, None)):
+        with pytest.raises((MaseAmdError, ValueError)):
+            c.append(key, value, counts=counts)
+        assert c._free == free and torch.equal(c._table, table) and [len(p) for p in c._pages] == [2, 0]
+        assert c.lengths() == [17, 0] and c._held_dev[0].tolist() == [0, 0]
