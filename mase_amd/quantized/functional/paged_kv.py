@@ -21,7 +21,7 @@ Arguments that all of them share:
 
 Lengths, slots and page numbers live on the device and are not looked at on the host (no call synchronizes, all can be
 captured into a graph): a length counts for at most ``max_length``, and a page number outside the pool is never followed,
-its slots being absent.  Inference only: no gradient is recorded.
+its slots being absent.  Inference only: tensors that record gradients are refused while gradients are enabled.
 """
 from __future__ import annotations
 
@@ -168,8 +168,8 @@ def _own_rows(t: Tensor, dtype: torch.dtype, batch: int, heads: int, least: int,
     return (n <= 1 or s1 == 1) and (heads == 1 or sh >= n) and (batch == 1 or sb >= (heads - 1) * (sh if heads > 1 else 0) + n)
 
 
-def _no_grad(what: str, *tensors: Tensor) -> None:
-    if any([t.requires_grad for t in tensors]) and torch.is_grad_enabled():
+def _no_grad(what: str, *tensors: Optional[Tensor]) -> None:
+    if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in tensors]):
         raise _lib.MaseAmdError(f"{what} is for inference and records no gradient: call it under torch.no_grad() or on detached tensors")
 
 
@@ -183,7 +183,7 @@ def paged_kv_append(key: Tensor, value: Tensor, k_pages: Tensor, v_pages: Tensor
     ``LinearMXFP`` do.  ``positions`` (int32 ``[batch, kv_heads, capacity]``, rows contiguous): entry slot becomes
     ``first_positions[b] + j`` (default ``starts[b] + j``).  Tokens without a slot in the table are not written."""
     what = "paged_kv_append"
-    _no_grad(what, key, value)
+    _no_grad(what, key, value, k_pages, v_pages)
     c = _Pool(what, k_pages, v_pages, page_table, kv_format, k_scales, v_scales, key.dtype)
     device = k_pages.device
     if key.dim() != 4 or value.shape != key.shape or value.dtype != key.dtype or (key.shape[0], key.shape[1], key.shape[3]) != (c.batch, c.kv_heads, c.head_dim):
@@ -220,6 +220,7 @@ def paged_kv_gather(k_pages: Tensor, v_pages: Tensor, page_table: Tensor, length
     """``(key, value)`` ``[batch, kv_heads, max_length, head_dim]`` of ``dtype`` (of the pages' type with
     ``kv_format=None``): the sequences' slots, zeros from ``lengths[b]`` (int32 ``[batch]``) on."""
     what = "paged_kv_gather"
+    _no_grad(what, k_pages, v_pages)
     if dtype is None:
         if kv_format is not None:
             raise ValueError(f"{what}: dtype is needed with kv_format={kv_format!r}")
@@ -252,7 +253,7 @@ def paged_attention_decode(query: Tensor, k_pages: Tensor, v_pages: Tensor, page
     ``[batch, kv_heads, >= max_length]``, rows contiguous): grows by the probabilities, summed over the query heads of each
     cached head.  ``max_length`` fixes how the work is split: one value for all calls of a captured step."""
     what = "paged_attention_decode"
-    _no_grad(what, query)
+    _no_grad(what, query, k_pages, v_pages, mask, weights)
     c = _Pool(what, k_pages, v_pages, page_table, kv_format, k_scales, v_scales, query.dtype)
     device, batch, kv_heads, head_dim = k_pages.device, c.batch, c.kv_heads, c.head_dim
     if query.dim() != 3 or query.shape[0] != batch or query.shape[2] != head_dim or query.shape[1] % kv_heads or query.shape[1] == 0:
@@ -306,6 +307,7 @@ def paged_kv_evict(k_pages: Tensor, v_pages: Tensor, page_table: Tensor, lengths
     ``paged_attention_decode`` and ``paged_kv_append``.  Returns new ``(weights, positions, lengths)``: what belongs to the
     slots now, zero and -1 behind.  A page must belong to one sequence only."""
     what = "paged_kv_evict"
+    _no_grad(what, k_pages, v_pages, weights)
     c = _Pool(what, k_pages, v_pages, page_table, kv_format, k_scales, v_scales,
               k_pages.dtype if kv_format is None else torch.bfloat16)
     device = k_pages.device

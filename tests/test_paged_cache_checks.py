@@ -1,4 +1,4 @@
-"""PagedKVCache on the host: masks over positions laid over slots, and what is refused before anything changes."""
+"""The paged cache on the host: masks over positions laid over slots, and what is refused before anything changes."""
 import pytest
 import torch
 
@@ -104,3 +104,27 @@ def test_a_refused_append_takes_no_pages():
             c.append(key, value, counts=counts)
         assert c._free == free and torch.equal(c._table, table) and [len(p) for p in c._pages] == [2, 0]
         assert c.lengths() == [17, 0] and c._held_dev[0].tolist() == [0, 0]
+
+
+def test_functions_refuse_whatever_records_gradients():
+    """pages, masks and weights like queries and states: none of the functions has a backward pass"""
+    from mase_amd._lib import MaseAmdError
+    from mase_amd.quantized import functional as F
+
+    k = torch.zeros(2, 1, 16, 64, dtype=torch.bfloat16)
+    kg = k.clone().requires_grad_()
+    t, n = torch.zeros(1, 1, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    x, q = torch.zeros(1, 1, 1, 64, dtype=torch.bfloat16), torch.zeros(1, 1, 64, dtype=torch.bfloat16)
+    m, w, pos = torch.zeros(1, 16), torch.zeros(1, 1, 16), torch.zeros(1, 1, 16, dtype=torch.int32)
+    grad = lambda t: t.clone().requires_grad_()  # noqa: E731
+    calls = [lambda: F.paged_kv_append(grad(x), x, k, k, t, n), lambda: F.paged_kv_append(x, grad(x), k, k, t, n)]
+    calls += [lambda: F.paged_attention_decode(grad(q), k, k, t, n, 16), lambda: F.paged_attention_decode(q, k, k, t, n, 16, mask=grad(m)),
+              lambda: F.paged_attention_decode(q, k, k, t, n, 16, weights=grad(w)), lambda: F.paged_kv_evict(k, k, t, n, grad(w), pos, 16, 8)]
+    for pages in ((kg, k), (k, kg)):
+        calls += [lambda p=pages: F.paged_kv_append(x, x, *p, t, n), lambda p=pages: F.paged_kv_gather(*p, t, n, 1),
+                  lambda p=pages: F.paged_attention_decode(q, *p, t, n, 16), lambda p=pages: F.paged_kv_evict(*p, t, n, w, pos, 16, 8)]
+    for call in calls:
+        with pytest.raises(MaseAmdError, match="gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(MaseAmdError, match="ROCm device"):
+            call()
