@@ -261,6 +261,8 @@ class PagedKVCache:
         self._refuse_capture("evict")
         if any(h != self._held[0] for h in self._held):
             raise ValueError("evict() comes between steps: the layers do not hold the same number of tokens")
+        if keep < 1 or recent < 0 or first < 0 or first + recent > keep:
+            raise ValueError(f"keep must be at least 1 and hold first + recent tokens, got keep={keep}, recent={recent}, first={first}")
         longest = max(self._held[0])
         if longest <= keep:
             return

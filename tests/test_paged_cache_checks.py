@@ -128,3 +128,13 @@ def test_functions_refuse_whatever_records_gradients():
             call()
         with torch.no_grad(), pytest.raises(MaseAmdError, match="ROCm device"):
             call()
+
+
+@pytest.mark.parametrize("keep,recent,first", [(0, 0, 0), (20, 21, 0), (20, -1, 0), (20, 0, -1), (20, 11, 10), (-3, 0, 0)])
+def test_evictions_that_cannot_be_are_refused_at_any_length(keep, recent, first):
+    c = cache([10, 10], [10, 10])
+    c.evict(20, recent=10, first=10)  # shorter than that: nothing to do
+    for held in ([10, 10], [0, 0]):
+        c._held = [held]
+        with pytest.raises(ValueError, match="keep"):
+            c.evict(keep, recent=recent, first=first)
