@@ -18,6 +18,8 @@ from torch import Tensor
 from .. import _lib
 from .functional import paged_kv as F
 
+_capturing = torch._C._cuda_isCurrentStreamCapturing
+
 # (kind, element bits or exponent and fraction bits) of the kv_cache quantizer that each code format holds the values of
 _FORMAT_OF = {("mxint", 8): "mxint8", ("mxfp", 4, 3): "mxfp8_e4m3", ("mxfp", 5, 2): "mxfp8_e5m2", ("mxfp", 2, 1): "mxfp4"}
 
@@ -61,6 +63,7 @@ class PagedKVCache:
             self._vs = torch.zeros((*shape[:3], head_dim // 32, page_size), dtype=torch.uint8, device=self.device)
         self._table = torch.full((batch_size, table_pages), -1, dtype=torch.int32, device=self.device)
         self.device = self._table.device  # with its index, whichever device is current later
+        self._on_gpu = self._table.is_cuda
         self._free = list(range(self.num_pages - 1, -1, -1))
         self._pages: List[List[int]] = [[] for _ in range(batch_size)]
         # per layer: slots held and tokens seen, on the host and on the device
@@ -166,12 +169,11 @@ class PagedKVCache:
         if len(new) != self.batch_size or any(c < 0 or c > n for c in new):
             raise ValueError(f"counts must be {self.batch_size} numbers from 0 to {n}, got {new}")
         held, seen = self._held[layer_idx], self._seen[layer_idx]
-        before = [len(p) for p in self._pages]
-        self._grow([h + c for h, c in zip(held, new)])
+        taken = self._grow([h + c for h, c in zip(held, new)])
         try:
             self._write(key_states, value_states, layer_idx, n, None if counts is None else new)
         except Exception:
-            self._give_back(before)  # a call that is refused takes no pages
+            self._give_back([len(p) - k for p, k in zip(self._pages, taken)])  # a call that is refused takes no pages
             raise
         for b, c in enumerate(new):
             held[b] += c
@@ -293,7 +295,7 @@ class PagedKVCache:
             raise ValueError(f"{what} needs a cache made with track_weights=True")
 
     def _refuse_capture(self, what: str) -> None:
-        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+        if self._on_gpu and _capturing():
             raise _lib.MaseAmdError(f"PagedKVCache.{what} cannot be captured into a graph, which would not move the lengths on the host: "
                                     "capture the functions of mase_amd.quantized.functional instead")
 
@@ -305,8 +307,8 @@ class PagedKVCache:
             return {}
         return dict(kv_format=self.kv_format, k_scales=self._ks[layer], v_scales=self._vs[layer])
 
-    def _grow(self, lengths: Sequence[int]) -> None:
-        """pages for sequences of these lengths"""
+    def _grow(self, lengths: Sequence[int]) -> List[int]:
+        """pages for sequences of these lengths; how many each of them took"""
         if max(lengths) > self.max_length:
             raise ValueError(f"a sequence of {max(lengths)} tokens does not fit a cache of max_length {self.max_length}")
         need = [max(0, -(-n // self.page_size) - len(p)) for n, p in zip(lengths, self._pages)]
@@ -319,6 +321,7 @@ class PagedKVCache:
                 got.append(self._free.pop())
                 self._pages[b].append(got[-1])
         self._set_table(at, got)
+        return need
 
     def _give_back(self, left: Sequence[int]) -> None:
         """the pages of each sequence behind its first left[b]"""
@@ -338,5 +341,5 @@ class PagedKVCache:
     def _staged(self, values) -> Tensor:
         """int64 numbers of the host on the device, in the order of the stream: a copy from pageable memory would wait for the
         GPU.  torch's allocator of pinned memory does not hand a block out again before the copies from it are done"""
-        host = torch.tensor(values, dtype=torch.int64, pin_memory=self.device.type == "cuda")
+        host = torch.tensor(values, dtype=torch.int64, pin_memory=self._on_gpu)
         return host.to(self.device, non_blocking=True)
