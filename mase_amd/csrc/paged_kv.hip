@@ -567,7 +567,7 @@ void launch_evict_move(const EvictParams& p, size_t batch, hipStream_t st) {
   hipLaunchKernelGGL((kv_evict_move_kernel<D, FMT>), grid, dim3(256), 0, st, p);
 }
 
-// calls F<D, FMT>::run(args...) for the pool's head dimension and format
+// calls fn<D, FMT>(args...) for the pool's head dimension and format
 #define MASE_KV_DISPATCH(cache, fn, ...)                                               \
   do {                                                                                 \
     switch ((int)(cache)->head_dim * 8 + (cache)->format) {                            \
@@ -702,8 +702,10 @@ extern "C" int mase_paged_kv_evict(const mase_paged_kv* cache, const int32_t* le
   p.first = (int)first;
   hipStream_t st = (hipStream_t)stream;
   const size_t most = max_length < capacity ? max_length : capacity;  // slots of a row
-  // short rows: fewer wavefronts, whose barriers are shorter
-  const int src = most <= 4096 ? launch_evict_select<4, true>(p, cache->batch, most, st)
+  // Short rows: four wavefronts, whose barriers are shorter; longer ones: sixteen, which have fewer turns.  Rows of 1024, 2048,
+  // 4096 and 8192 slots, 8 rows cut to half: 10.2, 11.3, 15.8 and 26.6 us with four, 12.3, 12.6, 13.3 and 14.9 with sixteen
+  // (64 rows alike).
+  const int src = most <= 2048 ? launch_evict_select<4, true>(p, cache->batch, most, st)
                   : most <= (size_t)kHeldSlots ? launch_evict_select<16, true>(p, cache->batch, most, st)
                                                : launch_evict_select<16, false>(p, cache->batch, most, st);
   if (src != MASE_OK) return src;
