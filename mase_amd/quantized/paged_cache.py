@@ -33,6 +33,8 @@ class PagedKVCache:
     sums of the attention weights are kept, which ``evict`` needs; ``attend`` adds to them, and so do the attention modules'
     dense steps (``add_weights``)."""
 
+    _most_sequences = 65535  # of one call of paged_attention_decode
+
     def __init__(self, batch_size: int, num_kv_heads: int, head_dim: int, max_length: int, num_layers: int = 1, *,
                  page_size: int = 64, num_pages: Optional[int] = None, kv_format: Optional[str] = None,
                  dtype: torch.dtype = torch.bfloat16, device="cuda", track_weights: bool = False):
@@ -239,21 +241,25 @@ class PagedKVCache:
                              f"position, got {mask.dtype} {tuple(mask.shape)}")
         if query.dim() != 3 or query.shape[0] != batch or query.shape[1] % heads:
             raise ValueError(f"query must be [{batch}, a multiple of {heads}, {self.head_dim}], got {tuple(query.shape)}")
-        if batch * heads > 65535:
-            raise ValueError(f"a mask after an eviction is for at most 65535 cached heads of sequences, got {batch * heads}")
         flat = mask.reshape(mask.shape[0], 1, mask.shape[-1]).expand(batch, heads, -1)
-        rows = flat.gather(-1, self._slot_positions(layer)).flatten(0, 1)
+        rows = flat.gather(-1, self._slot_positions(layer))
         single = lambda t: t.flatten(0, 1).unsqueeze(1)  # noqa: E731  [pages, heads, ...] as [pages * heads, 1, ...]
         head = torch.arange(heads, dtype=torch.int32, device=self.device)[:, None]
-        table = torch.where(self._table[:, None] < 0, -1, self._table[:, None] * heads + head).flatten(0, 1)
-        lengths = self._held_dev[layer].repeat_interleave(heads)
-        codes = self._codes(layer)
+        table = torch.where(self._table[:, None] < 0, -1, self._table[:, None] * heads + head)
+        lengths = self._held_dev[layer].repeat_interleave(heads).view(batch, heads)
+        k, v, codes = single(self._k[layer]), single(self._v[layer]), self._codes(layer)
         if codes:
             codes.update(k_scales=single(codes["k_scales"]), v_scales=single(codes["v_scales"]))
-        out = F.paged_attention_decode(query.reshape(batch * heads, -1, query.shape[2]), single(self._k[layer]), single(self._v[layer]),
-                                       table, lengths, max(self._held[layer]), scaling=scaling, mask=rows,
-                                       weights=single(self._weights[layer]), **codes)
-        return out.view(query.shape)
+        query = query.unflatten(1, (heads, -1))
+        parts = []
+        each = max(1, self._most_sequences // heads)
+        for lo in range(0, batch, each):
+            some = slice(lo, lo + each)
+            got = F.paged_attention_decode(query[some].flatten(0, 1), k, v, table[some].flatten(0, 1), lengths[some].flatten(),
+                                           max(self._held[layer]), scaling=scaling, mask=rows[some].flatten(0, 1),
+                                           weights=single(self._weights[layer][some]), **codes)
+            parts.append(got.view(-1, query.shape[1] * query.shape[2], self.head_dim))
+        return parts[0] if len(parts) == 1 else torch.cat(parts)
 
     # -- room ---------------------------------------------------------------------------------------------------------
     def evict(self, keep: int, *, recent: int = 0, first: int = 0) -> None:

@@ -136,10 +136,13 @@ def test_tokens_of_a_chunk_see_no_later_ones_after_an_eviction(dev, quantized):
     assert not torch.equal(a[-1]["y"][:, 3], b[-1]["y"][:, 3])
 
 
-def test_attend_takes_its_mask_by_positions(dev):
-    """the cache's own method: unequal lengths, an eviction, biases by position, weights"""
+@pytest.mark.parametrize("most", [65535, 4, 1])
+def test_attend_takes_its_mask_by_positions(dev, most, monkeypatch):
+    """the cache's own method: unequal lengths, an eviction, biases by position, weights; more cached heads of sequences than
+    one call takes"""
     from mase_amd.quantized import PagedKVCache
 
+    monkeypatch.setattr(PagedKVCache, "_most_sequences", most)
     g = torch.Generator().manual_seed(73)
     c = PagedKVCache(3, 2, 64, 80, page_size=16, kv_format="mxint8", dtype=DTYPE, device=dev, track_weights=True)
     kv = torch.randn(2, 3, 2, 40, 64, generator=g).to(DTYPE).to(dev)
