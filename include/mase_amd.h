@@ -472,7 +472,8 @@ int mase_paged_kv_gather(const mase_paged_kv* cache, const int32_t* lengths, siz
  * and sums are fp32; probabilities enter the product with the values as two numbers of `dtype`, the rounded one and the rest.
  * mask (optional): added to the scores of all heads, [batch][max_length] of mask_dtype (the cache's dtype or fp32) with an
  * element stride of batch (0: one row for all); a slot whose mask is -inf is left out whatever its keys and values hold.
- * A row without a slot gives zeros.  An infinite value in a slot that counts gives NaN.
+ * A row without a slot gives zeros.  An infinite value in a slot that counts gives NaN; sums are formed before the division
+ * by the softmax's, with terms of up to 2^8 times a value, so bf16 values beyond about 2^120 over the slots may overflow.
  * weights (optional, fp32) [batch][kv_heads][...] by element strides of batch and head: entry t grows by the probabilities
  * of slot t summed over the query heads of its cached head, in a fixed order.
  * The cache is split over its length; the parts (and with weights the scores) pass through `workspace`,

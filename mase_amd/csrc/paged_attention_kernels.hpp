@@ -1,7 +1,7 @@
 // Attention of one new token per sequence over a paged key-value cache for gfx950: x = scaling (q . k) + mask,
 // out = softmax(x) v, with the cache held in 16 bits or as MX codes (paged_kv.hpp).  The attention core of the reference's
 // Llama block on a cache (models/llama/modeling_llama.py:362-480, nn/quantized/modules/llama/attention.py:182-187, 352-395)
-// for one query.  Bound by HBM: every cached byte is read once.
+// for one query.  Bound by HBM: every cached byte is read once for each tile of 16 query heads of its cached head.
 //
 // One wavefront takes 32 slots at a time through two matrix products with up to 16 query heads of one cached head on the
 // other side, and no LDS: scores S^T = K Q^T (A = 16 key rows, B = the queries, both with 8 consecutive elements per lane),

@@ -136,7 +136,8 @@ __device__ __forceinline__ uint32_t encode8(const uint4& raw, const AppendParams
 // 16-bit rows: then the heads, then the tokens, the order in which projections leave their outputs (18381 tokens, 8 heads of
 // 128: 151 MB in 32.8 us; the other order 33.9).  Codes: then the tokens, then the heads, so that the scale bytes of the
 // values, which lie slot by slot, meet in a line (9227 tokens in MXINT8, 57 MB: 15.1 us; the other order 16.4).  Bound by
-// HBM for prompts, by the launch for single tokens (64 of them: 3 us).
+// HBM for prompts in 16 bits, nearly so in MXINT8, and by the launch for single tokens (64 of them: 3 us).  MXFP writes no more
+// bytes than MXINT8 but takes 30 us (e4m3), 28 (e5m2) and 24 (MXFP4) for the same tokens: the elements' arithmetic bounds it.
 template <int D, int FMT, int DT>
 __global__ __launch_bounds__(256) void kv_append_kernel(AppendParams p) {
   constexpr int kPieces = D / 8;
@@ -341,7 +342,7 @@ __device__ __forceinline__ void find_bin(uint32_t* hist, int want, int* sums, in
 // histograms over 8 bits of the keys each.  HELD: the row's keys stay in LDS (rows of up to kHeldSlots); otherwise
 // they are made anew from L2 for each pass.
 // It is bound by the latency of its dependent steps on one CU (two reads of the row, four histograms, the ranks): 39 us for
-// 64 rows of 20001 .. 32768 slots, 11 us for 8 rows of 2047.  Weights and positions are read in runs of independent loads
+// 64 rows of 20001 .. 32768 slots (30 MB, 6 us at the rate of a copy), 11 us for 8 rows of 2047.  Weights and positions are read in runs of independent loads
 // (one at a time, each waiting for L2: 103 us); keys in registers with every turn unrolled were no faster (45 us: the code
 // itself came from memory).
 constexpr int kHeldSlots = 36864;
@@ -522,8 +523,9 @@ int launch_evict_select(const EvictParams& p, size_t batch, size_t most, hipStre
 }
 
 // Moves kept rows from behind `keep` into the free slots: sources and targets are disjoint, so the order does not matter, and
-// only rows that change place are touched.  16 bytes of keys and of values per lane.  Bound by HBM: 8 x 8 heads of
-// 20001 .. 32768 MXINT8 rows of 128 cut to 16384, about 0.4 GB, 50 us.
+// only rows that change place are touched.  16 bytes of keys and of values per lane.  8 x 8 heads of 20001 .. 32768 MXINT8
+// rows of 128 cut to 16384: 380 thousand rows of 264 bytes read and written, 0.20 GB in 50 us, 4.0 TB/s where a large copy
+// moves 4.9: single rows here and there, and the values' scale bytes one by one.
 template <int D, int FMT>
 __global__ __launch_bounds__(256) void kv_evict_move_kernel(EvictParams p) {
   constexpr int kRow = FMT == MASE_KV_16BIT ? 2 * D : (FMT == MASE_KV_MXFP4 ? D / 2 : D);

@@ -249,7 +249,8 @@ def paged_attention_decode(query: Tensor, k_pages: Tensor, v_pages: Tensor, page
     ``scaling`` defaults to ``head_dim ** -0.5``.  ``mask``: added to the scores of every head, ``[batch or 1, >= max_length]``
     of ``query``'s type or float32 (also with dimensions of size one in between, as the 4-D masks of the attention modules
     have); a slot masked with -inf is left out whatever it holds.  A row without slots gives zeros; an
-    infinite value in a slot that counts gives NaN.  ``weights`` (float32
+    infinite value in a slot that counts gives NaN (sums are formed before the division: bf16 values beyond about 2^120 over
+    the number of slots may overflow).  ``weights`` (float32
     ``[batch, kv_heads, >= max_length]``, rows contiguous): grows by the probabilities, summed over the query heads of each
     cached head.  ``max_length`` fixes how the work is split: one value for all calls of a captured step."""
     what = "paged_attention_decode"
