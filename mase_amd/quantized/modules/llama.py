@@ -191,7 +191,7 @@ class _LlamaAttentionMX(nn.Module):
             paged = isinstance(past_key_value, PagedKVCache)
             if paged:
                 past_key_value.require_kind(None if self.kv_cache_bypass else self._kind, self.kv_cache_config)
-                past_key_value.require_mask(attention_mask, query_states.shape[2], self.layer_idx)
+                past_key_value.require_mask(attention_mask, query_states.shape[2], self.layer_idx, query_states.shape[1])
                 if self._reads_pages(query_states, attention_mask):
                     return self._attend_pages(past_key_value, query_states, key_states, value_states, attention_mask, input_shape)
             # a packed paged cache quantizes what it writes

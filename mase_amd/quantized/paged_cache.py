@@ -3,7 +3,7 @@
 It takes the place of the cache object that the attention modules call ``past_key_value.update`` on
 (``chop/nn/quantized/modules/llama/attention.py:182-187``): ``update`` appends and returns the dense states, ``append`` and
 ``attend`` do a decoding step on the pages alone, and ``evict`` cuts the sequences down to a budget by the attention
-weights that ``attend`` has added up.  The functions underneath are in ``mase_amd.quantized.functional``.
+weights that the steps have added up.  The functions underneath are in ``mase_amd.quantized.functional``.
 
 The host keeps how long each sequence is, so no call waits for the GPU; a replayed graph would not move that on, so no
 call can be captured: a step that is captured uses the functions directly, with lengths that the graph itself moves on.
@@ -29,9 +29,8 @@ class PagedKVCache:
 
     ``kv_format``: None (states of ``dtype``), ``"mxint8"``, ``"mxfp8_e4m3"``, ``"mxfp8_e5m2"`` or ``"mxfp4"`` (blocks of 32
     along the head dimension).  ``num_pages`` (default: enough for every sequence at ``max_length``) is the pool's size for
-    each layer; a sequence takes pages as it grows.  ``track_weights``: positions and the
-    sums of the attention weights are kept, which ``evict`` needs; ``attend`` adds to them, and so do the attention modules'
-    dense steps (``add_weights``)."""
+    each layer; a sequence takes pages as it grows.  ``track_weights``: positions and the sums of the attention weights are
+    kept, which ``evict`` needs; ``attend`` adds to them, and so do the attention modules' dense steps (``add_weights``)."""
 
     _most_sequences = 65535  # of one call of paged_attention_decode
 
@@ -115,9 +114,10 @@ class PagedKVCache:
     def _evicted(self, layer: int) -> bool:
         return self._held[layer] != self._seen[layer]
 
-    def require_mask(self, mask: Optional[Tensor], tokens: int, layer_idx: int = 0) -> None:
+    def require_mask(self, mask: Optional[Tensor], tokens: int, layer_idx: int = 0, heads: Optional[int] = None) -> None:
         """raises ValueError unless ``mask`` (``[batch or 1, heads or 1, tokens or 1, columns]``, added to the scores of the
-        next ``tokens`` tokens, one column for each position) can be laid over the layer's slots once they are appended"""
+        next ``tokens`` tokens, one column for each position) can be laid over the layer's slots once they are appended;
+        ``heads``: of the queries"""
         evicted, seen = self._evicted(layer_idx), self._seen[layer_idx]
         if mask is not None and min(seen) != max(seen):
             raise ValueError("a mask with one column for each position needs sequences that stand at the same one: these have seen "
@@ -127,7 +127,8 @@ class PagedKVCache:
         total = self.get_seq_length(layer_idx) + tokens
         fits = mask.dim() == 4 and mask.shape[0] in (1, self.batch_size) and mask.shape[3] >= total
         if fits and evicted:
-            fits = mask.is_floating_point() and mask.shape[2] in (1, tokens) and (mask.shape[1] == 1 or mask.shape[1] % self.num_kv_heads == 0)
+            each = mask.shape[1] % self.num_kv_heads == 0 if heads is None else mask.shape[1] == heads
+            fits = mask.is_floating_point() and mask.shape[2] in (1, tokens) and (mask.shape[1] == 1 or each)
         if not fits:
             raise ValueError(f"mask must be a floating-point tensor [{self.batch_size} or 1, heads or 1, {tokens} or 1, at least {total}] with "
                              f"one column for each position, got {mask.dtype} {tuple(mask.shape)}")
@@ -136,8 +137,11 @@ class PagedKVCache:
         """the mask over the rows that ``gather`` returns, of one whose columns are positions: the same one until the layer
         is evicted from, then ``[batch, heads, rows, longest]``.  The zeros behind shorter sequences are hidden by the type's
         lowest value (without a mask: by one of the states' type, ``[batch, 1, 1, longest]``)"""
-        held = self._held[layer_idx]
-        if mask is not None and self._evicted(layer_idx):
+        held, seen = self._held[layer_idx], self._seen[layer_idx]
+        if mask is not None and held != seen:
+            # the position of every slot has to be a column
+            if mask.dim() != 4 or not mask.is_floating_point() or mask.shape[0] not in (1, self.batch_size) or mask.shape[1] not in (1, heads) or mask.shape[3] < max(seen):
+                raise ValueError(f"mask must be a floating-point tensor [{self.batch_size} or 1, {heads} or 1, rows, at least {max(seen)}], got {mask.dtype} {tuple(mask.shape)}")
             mask = self._gather_columns(mask, heads, layer_idx)
         if min(held) == max(held):
             return mask
@@ -239,7 +243,7 @@ class PagedKVCache:
                 or mask.dtype not in (self.dtype, torch.float32)):
             raise ValueError(f"mask must be {self.dtype} or float32 [{batch} or 1, (1, ...) at least {columns}] with one column for each "
                              f"position, got {mask.dtype} {tuple(mask.shape)}")
-        if query.dim() != 3 or query.shape[0] != batch or query.shape[1] % heads:
+        if query.dim() != 3 or query.shape[0] != batch or query.shape[1] % heads or query.shape[1] == 0:
             raise ValueError(f"query must be [{batch}, a multiple of {heads}, {self.head_dim}], got {tuple(query.shape)}")
         flat = mask.reshape(mask.shape[0], 1, mask.shape[-1]).expand(batch, heads, -1)
         rows = flat.gather(-1, self._slot_positions(layer))

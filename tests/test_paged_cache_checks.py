@@ -138,3 +138,17 @@ def test_evictions_that_cannot_be_are_refused_at_any_length(keep, recent, first)
         c._held = [held]
         with pytest.raises(ValueError, match="keep"):
             c.evict(keep, recent=recent, first=first)
+
+
+@pytest.mark.parametrize("bad", [torch.zeros(2, 1, 3, 23), torch.zeros(2, 4, 3, 24), torch.zeros(3, 1, 3, 24), torch.zeros(2, 3, 24),
+                                 torch.zeros(2, 1, 3, 24, dtype=torch.bool)])
+def test_no_position_is_looked_up_past_a_mask(bad):
+    """an index past the columns would end a kernel, and with it the process"""
+    held, seen = [10, 10], [24, 24]
+    c = cache(held, seen, scattered(held, seen, 2, 32, torch.Generator().manual_seed(112)))
+    assert c.slot_mask(torch.zeros(2, 6, 3, 24), 6).shape == (2, 6, 3, 10)
+    with pytest.raises(ValueError, match="mask"):
+        c.slot_mask(bad, 6)
+    c.require_mask(torch.zeros(2, 6, 1, 25), 1, heads=6)
+    with pytest.raises(ValueError, match="mask"):
+        c.require_mask(torch.zeros(2, 4, 1, 25), 1, heads=6)
